@@ -5,6 +5,7 @@
 The library lands where the reference's Python looks for it relative to its scripts folder
 (<root>/build/libg1env.so, reference scripts/ppo.py:20-24), with <root> = g1.cu_amd.
 """
+import concurrent.futures
 import json
 import os
 import re
@@ -31,7 +32,7 @@ FLAGS = [
 ]
 
 
-# translation units and their own flags: both are scheduled for instruction-level parallelism with
+# translation units and their own flags: those of the environment are scheduled for instruction-level parallelism with
 # LLVM's max-ilp machine scheduler. k_physics and k_policy since the physics lost its force
 # broadcast and select cascades (config 4 rollout 185.4 -> 183.5 ms; with the older physics the
 # same flag had made it 3% slower); the iterative ILP scheduler measured 2.5% slower and the default
@@ -48,6 +49,9 @@ SOURCES = (
     ("g1env.hip", ILP_FIRST),
     ("rollout_kernel.hip", ILP_FIRST + MFMA_VGPR),
     ("resident_kernel.hip", ILP_FIRST),
+    ("nn_norm.hip", []),
+    ("nn_clip.hip", []),
+    ("nn_gated.hip", []),
 )
 
 
@@ -71,17 +75,24 @@ def _parse_resources(text, table):
             table[fn][key.split(" [")[0]] = int(val)
 
 
+def _compile(name, extra):
+    """One translation unit: (object, compiler's output)."""
+    obj = os.path.join(OUT_DIR, os.path.splitext(name)[0] + ".o")
+    cmd = ["hipcc", *FLAGS, *extra, "-Rpass-analysis=kernel-resource-usage", "-c", os.path.join(HERE, "csrc", name),
+           "-o", obj]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    return obj, cmd, p
+
+
 def build(verbose=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     objs = []
     resources = {}
-    for name, extra in SOURCES:
-        obj = os.path.join(OUT_DIR, os.path.splitext(name)[0] + ".o")
-        cmd = ["hipcc", *FLAGS, *extra, "-Rpass-analysis=kernel-resource-usage", "-c",
-               os.path.join(HERE, "csrc", name), "-o", obj]
+    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        done = list(pool.map(lambda s: _compile(*s), SOURCES))
+    for obj, cmd, p in done:
         if verbose:
             print(" ".join(cmd), flush=True)
-        p = subprocess.run(cmd, capture_output=True, text=True)
         if p.returncode != 0 or verbose:
             sys.stderr.write(p.stdout + p.stderr)
         if p.returncode != 0:

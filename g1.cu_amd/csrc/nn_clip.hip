@@ -1,0 +1,173 @@
+// nn_clip.hip -- the global norm of many gradient tensors, and the tensors clipped to it:
+//   norm = sqrt(sum of all squares);  out = in * min(1, max_norm / (norm + 1e-6))
+//
+// Two launches per table of tensors: the blocks' sums of squares, in 64 bits (a square of any finite 32-bit value
+// fits, so the norm overflows only where it is itself too large), and the scaling, whose blocks each join those sums in
+// the same fixed order. Bound by memory: the tensors are read twice and written once.
+#include <algorithm>
+
+#include "../../include/g1nn.h"
+#include "nn_common.h"
+
+namespace g1nn {
+
+constexpr int kTable = 64;          // tensors of one launch: their table travels as a kernel argument
+constexpr int kClipThreads = 256;
+constexpr int kChunk = 16384;       // elements of a block's turn
+constexpr int kSums = 1024;         // sums of one launch: its largest grid
+
+struct ClipTable {
+  int n, chunks;
+  const void* in[kTable];
+  void* out[kTable];
+  long size[kTable];
+  int first[kTable + 1];            // the first chunk of each tensor
+  unsigned char in_type[kTable], out_type[kTable];
+};
+
+__device__ __forceinline__ int tensor_of(const ClipTable& t, int chunk) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (t.first[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* part) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int i = 1; i < kClipThreads / 64; i++) v += part[i];
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ double squares(const T* p, long n) {
+  constexpr int V = 16 / sizeof(T);
+  double s = 0;
+  long i = 0;
+  if (((uintptr_t)p & 15) == 0) {
+    for (i = (long)threadIdx.x * V; i + V <= n; i += kClipThreads * V) {
+      float v[V];
+      Elems<T, V>::load(p + i, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) s += (double)v[j] * (double)v[j];
+    }
+    i = n / V * V;
+  }
+  for (i += threadIdx.x; i < n; i += kClipThreads) s += (double)(float)p[i] * (double)(float)p[i];
+  return s;
+}
+
+__global__ __launch_bounds__(kClipThreads) void k_clip_sums(ClipTable t, double* sums) {
+  __shared__ double part[kClipThreads / 64];
+  double s = 0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int i = tensor_of(t, c);
+    const long at = (long)(c - t.first[i]) * kChunk, left = t.size[i] - at, n = left < kChunk ? left : kChunk;
+    s += t.in_type[i] == 0 ? squares((const float*)t.in[i] + at, n) : squares((const bf16*)t.in[i] + at, n);
+  }
+  s = block_sum(s, part);
+  if (threadIdx.x == 0) sums[blockIdx.x] = s;
+}
+
+template <typename I, typename O>
+__device__ __forceinline__ void scale(const I* in, O* out, long n, float f) {
+  constexpr int V = 16 / (sizeof(I) < sizeof(O) ? sizeof(O) : sizeof(I));
+  long i = 0;
+  if ((((uintptr_t)in & (V * sizeof(I) - 1)) | ((uintptr_t)out & (V * sizeof(O) - 1))) == 0) {
+    for (i = (long)threadIdx.x * V; i + V <= n; i += kClipThreads * V) {
+      float v[V];
+      Elems<I, V>::load(in + i, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] *= f;
+      Elems<O, V>::store(out + i, v);
+    }
+    i = n / V * V;
+  }
+  for (i += threadIdx.x; i < n; i += kClipThreads) out[i] = (O)((float)in[i] * f);
+}
+
+__global__ __launch_bounds__(kClipThreads) void k_clip_scale(ClipTable t, const double* sums, int nsums, float max_norm,
+                                                              float* norm) {
+  __shared__ double part[kClipThreads / 64];
+  double s = 0;
+  for (int i = threadIdx.x; i < nsums; i += kClipThreads) s += sums[i];
+  const float total = (float)sqrt(block_sum(s, part));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  float f = max_norm / (total + 1e-6f);
+  f = f > 1.0f ? 1.0f : f;   // a NaN stays one
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int i = tensor_of(t, c);
+    const long at = (long)(c - t.first[i]) * kChunk, left = t.size[i] - at, n = left < kChunk ? left : kChunk;
+    const void* in = t.in[i];
+    void* out = t.out[i];
+    const int it = t.in_type[i], ot = t.out_type[i];
+    if (in == out && f == 1.0f) continue;
+    if (it == 0 && ot == 0) scale((const float*)in + at, (float*)out + at, n, f);
+    else if (it == 0) scale((const float*)in + at, (bf16*)out + at, n, f);
+    else if (ot == 0) scale((const bf16*)in + at, (float*)out + at, n, f);
+    else scale((const bf16*)in + at, (bf16*)out + at, n, f);
+  }
+}
+
+}  // namespace g1nn
+
+using namespace g1nn;
+
+extern "C" long g1_nn_clip_workspace(int n) {
+  const long launches = n > 0 ? (n + kTable - 1) / kTable : 1;
+  return launches * kSums * (long)sizeof(double);
+}
+
+extern "C" int g1_nn_clip(int n, const void* const* in, const int* in_type, void* const* out, const int* out_type,
+                          const long* size, float max_norm, float* norm, void* ws, void* stream) {
+  const hipStream_t st = (hipStream_t)stream;
+  if (n < 0 || (n > 0 && (!in || !in_type || !out || !out_type || !size))) return refuse("a null table") ? -1 : 0;
+  if (!norm || !ws || !aligned(ws, 16)) return refuse("the norm and a 16-byte aligned workspace are needed") ? -1 : 0;
+  if (!(max_norm >= 0)) return refuse("max_norm is a number of at least 0") ? -1 : 0;
+  for (int i = 0; i < n; i++) {
+    if ((in_type[i] != 0 && in_type[i] != 1) || (out_type[i] != 0 && out_type[i] != 1))
+      return refuse("type is 0 (fp32) or 1 (bf16)") ? -1 : 0;
+    if (size[i] < 0 || size[i] > (1l << 44)) return refuse("a tensor's size is out of range") ? -1 : 0;
+    if (size[i] > 0 && (!in[i] || !out[i])) return refuse("a null pointer") ? -1 : 0;
+    if (!aligned(in[i], in_type[i] == 0 ? 4 : 2) || !aligned(out[i], out_type[i] == 0 ? 4 : 2))
+      return refuse("an address is not aligned to its elements") ? -1 : 0;
+    if (size[i] > 0 && in[i] == out[i] && in_type[i] != out_type[i]) return refuse("in place, the types are the same") ? -1 : 0;
+  }
+  double* sums = (double*)ws;
+  int nsums = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    for (int from = 0; from < n || from == 0; from += kTable) {
+      ClipTable t;
+      t.n = std::min(kTable, n - from);
+      long chunks = 0;
+      for (int i = 0; i < t.n; i++) {
+        t.in[i] = in[from + i];
+        t.out[i] = out[from + i];
+        t.size[i] = size[from + i];
+        t.in_type[i] = (unsigned char)in_type[from + i];
+        t.out_type[i] = (unsigned char)out_type[from + i];
+        t.first[i] = (int)chunks;
+        chunks += (size[from + i] + kChunk - 1) / kChunk;
+        if (chunks > 0x7fffffff) return refuse("the tensors are too large") ? -1 : 0;
+      }
+      t.first[t.n] = t.chunks = (int)chunks;
+      const int grid = std::max(1, (int)std::min<long>(chunks, pass == 0 ? kSums : 2048));
+      int rc;
+      if (pass == 0) {
+        rc = launch(k_clip_sums, dim3(grid), dim3(kClipThreads), st, t, sums + nsums);
+        nsums += grid;
+      } else {
+        rc = launch(k_clip_scale, dim3(grid), dim3(kClipThreads), st, t, sums, nsums, max_norm, from == 0 ? norm : nullptr);
+      }
+      if (rc) return rc;
+    }
+  }
+  return 0;
+}

@@ -1,0 +1,76 @@
+// nn_common.h -- what the policy operators' kernels share: element types, 16-byte accesses, reductions over the
+// lanes of a row, and the C entries' checks.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <tuple>
+
+namespace g1nn {
+
+typedef __bf16 bf16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// One access of VEC elements (16 bytes for the vector forms), as floats.
+template <typename T, int VEC>
+struct Elems {
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  static __device__ __forceinline__ void load(const T* p, float (&o)[VEC]) {
+    const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) o[i] = (float)v[i];
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&o)[VEC]) {
+    V v;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) v[i] = (T)o[i];
+    *reinterpret_cast<V*>(p) = v;
+  }
+};
+template <typename T>
+struct Elems<T, 1> {
+  static __device__ __forceinline__ void load(const T* p, float (&o)[1]) { o[0] = (float)*p; }
+  static __device__ __forceinline__ void store(T* p, const float (&o)[1]) { *p = (T)o[0]; }
+};
+
+// Sum (or largest) over the TPR threads that share a row: butterflies within a wave, then the waves' values through
+// LDS. `part` has 2 x 16 values and is used alternately (`turn`), so one barrier per reduction is enough: the next
+// one writes the other half, and the one after it is behind that one's barrier.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* part, int turn) {
+#pragma unroll
+  for (int d = 1; d < (TPR < 64 ? TPR : 64); d *= 2) v += __shfl_xor(v, d);
+  if (TPR > 64) {
+    float* p = part + (turn & 1) * 16;
+    if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = p[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; i++) v += p[i];
+  }
+  return v;
+}
+
+inline bool refuse(const char* what) {
+  fprintf(stderr, "g1nn: %s\n", what);
+  return true;
+}
+
+// Enqueue a kernel with arguments of its own parameter types: 0, or -2 with a message. The status is this launch's own,
+// not an error that something else left behind.
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t st, A... args) {
+  std::tuple<P...> held(args...);
+  void* at[sizeof...(P)];
+  int n = 0;
+  std::apply([&](auto&... v) { ((at[n++] = (void*)&v), ...); }, held);
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, at, 0, st);
+  if (e == hipSuccess) return 0;
+  fprintf(stderr, "g1nn HIP error: %s\n", hipGetErrorString(e));
+  return -2;
+}
+
+inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+}  // namespace g1nn

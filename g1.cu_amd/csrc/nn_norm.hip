@@ -1,0 +1,357 @@
+// nn_norm.hip -- root-mean-square norm of a residual stream: forward with the residual's addition, the same with rows
+// in 8 bits, and the gradients.
+//
+//   h = x + r;  s = 1 / sqrt(mean(h^2) + eps);  y = h s w
+//   dx = dr = s (dy w - h s^2 mean(dy w h)) + dh;  dw = sum over rows of dy h s
+//   8 bits: u = h w, a = max|u|, q = rint(u 127/a), scale = (a / 127) s
+//
+// All of them move each value once and are bound by memory: a row stays in the registers of the TPR threads that share
+// it (16 lanes to a whole block, by the row's length) between the reduction and the store.
+#include "../../include/g1nn.h"
+#include "nn_common.h"
+
+namespace g1nn {
+
+constexpr int kMaxRow = 32768;
+
+struct NormArgs {
+  long M;
+  int K;
+  const void *x, *r, *w;
+  long xs, rs;
+  float eps;
+  void *y, *h;
+  float* rstd;   // the 8-bit form: the scales
+};
+
+template <typename T, int VEC, int TPR, int NV, bool Q8>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) {
+  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
+  __shared__ float part[32];
+  __shared__ unsigned most[32];
+  const int lane = threadIdx.x % TPR;
+  float w[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int k = (i * TPR + lane) * VEC;
+    if (k < a.K) Elems<T, VEC>::load((const T*)a.w + k, w[i]);
+  }
+  int turn = 0;
+  // every thread of a block makes the same number of turns where the block shares a row (kRows = 1)
+  for (long row = (long)blockIdx.x * kRows + threadIdx.x / TPR; row < a.M; row += (long)gridDim.x * kRows, turn++) {
+    const T* x = (const T*)a.x + row * a.xs;
+    const T* r = a.r ? (const T*)a.r + row * a.rs : nullptr;
+    float h[NV][VEC];
+    float sq = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int k = (i * TPR + lane) * VEC;
+      if (k < a.K) {
+        Elems<T, VEC>::load(x + k, h[i]);
+        if (r) {
+          float e[VEC];
+          Elems<T, VEC>::load(r + k, e);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) h[i][j] += e[j];
+          Elems<T, VEC>::store((T*)a.h + row * a.K + k, h[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; j++) sq = __builtin_fmaf(h[i][j], h[i][j], sq);
+      }
+    }
+    sq = row_sum<TPR>(sq, part, turn);
+    const float s = 1.0f / sqrtf(sq / (float)a.K + a.eps);
+    if (!Q8) {
+      if (a.rstd && lane == 0) a.rstd[row] = s;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int k = (i * TPR + lane) * VEC;
+        if (k < a.K) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) h[i][j] = h[i][j] * s * w[i][j];
+          Elems<T, VEC>::store((T*)a.y + row * a.K + k, h[i]);
+        }
+      }
+    } else {
+      // the largest |u| by its bits: as whole numbers they order like the values, infinities and NaN above them
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int k = (i * TPR + lane) * VEC;
+        if (k < a.K) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) {
+            h[i][j] *= w[i][j];
+            const unsigned b = __float_as_uint(h[i][j]) & 0x7fffffffu;
+            top = b > top ? b : top;
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < (TPR < 64 ? TPR : 64); d *= 2) {
+        const unsigned o = __shfl_xor(top, d);
+        top = o > top ? o : top;
+      }
+      if (TPR > 64) {
+        unsigned* p = most + (turn & 1) * 16;
+        if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPR / 64; i++) top = p[i] > top ? p[i] : top;
+      }
+      const float amax = __uint_as_float(top);
+      float inv = 127.0f / amax, scale = (amax / 127.0f) * s;
+      if (top >= 0x7f800000u) {
+        inv = 0;
+        scale = __uint_as_float(0x7fc00000u);
+      } else if (__float_as_uint(inv) >= 0x7f800000u) {
+        inv = 0;
+        scale = 0;
+      }
+      if (lane == 0) a.rstd[row] = scale;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int k = (i * TPR + lane) * VEC;
+        if (k < a.K) {
+          typedef signed char B __attribute__((ext_vector_type(VEC == 1 ? 2 : VEC)));
+          B b;
+#pragma unroll
+          for (int j = 0; j < VEC; j++) b[j] = inv == 0 ? 0 : (signed char)(int)rintf(h[i][j] * inv);
+          signed char* q = (signed char*)a.y + row * a.K + k;
+          if (VEC == 1) *q = b[0];
+          else *reinterpret_cast<B*>(q) = b;
+        }
+      }
+    }
+  }
+}
+
+struct NormGradArgs {
+  long M;
+  int K;
+  const void *dy, *dh, *h, *w;
+  long dys, dhs, hs;
+  const float* rstd;
+  void* dx;
+  float* dw;   // [gridDim.x][K] sums of a block's rows, or null
+};
+
+template <typename T, int VEC, int TPR, int NV>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGradArgs a) {
+  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
+  __shared__ float part[32];
+  __shared__ float cols[kRows > 1 ? kBlock * VEC * NV : 1];
+  const int lane = threadIdx.x % TPR;
+  float w[NV][VEC], dw[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int k = (i * TPR + lane) * VEC;
+    if (k < a.K) Elems<T, VEC>::load((const T*)a.w + k, w[i]);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) dw[i][j] = 0;
+  }
+  int turn = 0;
+  for (long row = (long)blockIdx.x * kRows + threadIdx.x / TPR; row < a.M; row += (long)gridDim.x * kRows, turn++) {
+    const T* dy = (const T*)a.dy + row * a.dys;
+    const T* hp = (const T*)a.h + row * a.hs;
+    const float s = a.rstd[row];
+    float g[NV][VEC], h[NV][VEC];
+    float c = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int k = (i * TPR + lane) * VEC;
+      if (k < a.K) {
+        Elems<T, VEC>::load(dy + k, g[i]);
+        Elems<T, VEC>::load(hp + k, h[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          h[i][j] *= s;
+          dw[i][j] = __builtin_fmaf(g[i][j], h[i][j], dw[i][j]);
+          g[i][j] *= w[i][j];
+          c = __builtin_fmaf(g[i][j], h[i][j], c);
+        }
+      }
+    }
+    c = row_sum<TPR>(c, part, turn) / (float)a.K;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int k = (i * TPR + lane) * VEC;
+      if (k < a.K) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) g[i][j] = s * __builtin_fmaf(-h[i][j], c, g[i][j]);
+        if (a.dh) {
+          float e[VEC];
+          Elems<T, VEC>::load((const T*)a.dh + row * a.dhs + k, e);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) g[i][j] += e[j];
+        }
+        Elems<T, VEC>::store((T*)a.dx + row * a.K + k, g[i]);
+      }
+    }
+  }
+  if (!a.dw) return;
+  // the block's rows joined in a fixed order
+  if (kRows > 1) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) cols[(i * VEC + j) * kBlock + threadIdx.x] = dw[i][j];
+    __syncthreads();
+    if (threadIdx.x >= TPR) return;
+    for (int o = 1; o < kRows; o++)
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) dw[i][j] += cols[(i * VEC + j) * kBlock + o * TPR + lane];
+  }
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int k = (i * TPR + lane) * VEC;
+    if (k < a.K)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) a.dw[(long)blockIdx.x * a.K + k + j] = dw[i][j];
+  }
+}
+
+// dw [K] from the blocks' P rows of sums: 32 columns to a block, its eight groups of lanes each taking every eighth row
+template <typename T>
+__global__ __launch_bounds__(256) void k_column_join(const float* part, int P, int K, T* out) {
+  __shared__ float s[8][32];
+  const int c = threadIdx.x & 31, o = threadIdx.x >> 5, k = blockIdx.x * 32 + c;
+  float v = 0;
+  if (k < K)
+    for (int p = o; p < P; p += 8) v += part[(long)p * K + k];
+  s[o][c] = v;
+  __syncthreads();
+  if (o == 0 && k < K) {
+    for (int i = 1; i < 8; i++) v += s[i][c];
+    out[k] = (T)v;
+  }
+}
+
+// The forms (threads per row, accesses per thread): the fewest threads whose registers hold the row in a few accesses
+// each. VEC = 1 takes rows that 16-byte accesses do not fit (odd lengths, strides or addresses).
+template <typename T, int VEC, typename F>
+int by_row(int K, F f) {
+  const int n = (K + VEC - 1) / VEC;
+  if (n <= 16) return f.template go<T, VEC, 16, 1>();
+  if (n <= 64) return f.template go<T, VEC, 64, 1>();
+  if (n <= 128) return f.template go<T, VEC, 64, 2>();
+  if (n <= 256) return f.template go<T, VEC, 64, 4>();
+  if (n <= 1024) return f.template go<T, VEC, 256, 4>();
+  if (n <= 2048) return f.template go<T, VEC, 256, 8>();
+  if (n <= 8192) return f.template go<T, VEC, 1024, 8>();
+  if (VEC == 1) return f.template go<T, 1, 1024, 32>();
+  return -1;
+}
+
+template <typename F>
+int by_type(int type, bool wide, int K, F f) {
+  if (type == 0) return wide ? by_row<float, 4>(K, f) : by_row<float, 1>(K, f);
+  return wide ? by_row<bf16, 8>(K, f) : by_row<bf16, 1>(K, f);
+}
+
+constexpr long kGrid = 2048;       // blocks of a forward launch: eight to a CU
+constexpr long kGradGrid = 1024;   // of a backward launch, each of which leaves one row of sums for dw
+
+inline long grid_for(long M, int rows, long most) {
+  const long n = (M + rows - 1) / rows;
+  return n < most ? n : most;
+}
+
+template <bool Q8>
+struct Forward {
+  const NormArgs& a;
+  hipStream_t st;
+  template <typename T, int VEC, int TPR, int NV>
+  int go() {
+    constexpr int kBlock = TPR > 256 ? TPR : 256;
+    return launch(k_rms_norm<T, VEC, TPR, NV, Q8>, dim3(grid_for(a.M, kBlock / TPR, kGrid)), dim3(kBlock), st, a);
+  }
+};
+
+struct Backward {
+  const NormGradArgs& a;
+  hipStream_t st;
+  long* grid;
+  template <typename T, int VEC, int TPR, int NV>
+  int go() {
+    constexpr int kBlock = TPR > 256 ? TPR : 256;
+    *grid = grid_for(a.M, kBlock / TPR, kGradGrid);
+    return launch(k_rms_norm_grad<T, VEC, TPR, NV>, dim3(*grid), dim3(kBlock), st, a);
+  }
+};
+
+inline bool bad_shape(int type, long M, int K) {
+  if (type != 0 && type != 1) return refuse("type is 0 (fp32) or 1 (bf16)");
+  if (M < 0) return refuse("a negative number of rows");
+  if (K < 1 || K > kMaxRow) return refuse("rows of 1 to 32768 values are supported");
+  return false;
+}
+
+inline bool fits(int type, int K, const void* p, long stride) {
+  const int vec = type == 0 ? 4 : 8;
+  return !p || (aligned(p, 16) && stride % vec == 0);
+}
+
+inline bool bad_rows(const void* p, int type) {
+  return !aligned(p, type == 0 ? 4 : 2) && refuse("an address is not aligned to its elements");
+}
+
+template <bool Q8>
+int forward(int type, long M, int K, const void* x, long xs, const void* r, long rs, const void* w, float eps, void* y,
+            void* h, float* rstd, hipStream_t st) {
+  if (bad_shape(type, M, K)) return -1;
+  if (M == 0) return 0;
+  if (!x || !w || !y || (Q8 && !rstd)) return refuse("a null pointer") ? -1 : 0;
+  if (!r != !h) return refuse("the new stream h goes with the residual r") ? -1 : 0;
+  if (bad_rows(x, type) || bad_rows(r, type) || bad_rows(w, type) || bad_rows(h, type) || (!Q8 && bad_rows(y, type)))
+    return -1;
+  const NormArgs a{M, K, x, r, w, xs, rs, eps, y, h, rstd};
+  const int vec = type == 0 ? 4 : 8;
+  const bool wide = K % vec == 0 && fits(type, K, x, xs) && fits(type, K, r, rs) && fits(type, K, w, K) &&
+                    fits(type, K, h, K) && (Q8 ? aligned(y, vec) : fits(type, K, y, K));
+  return by_type(type, wide, K, Forward<Q8>{a, st});
+}
+
+}  // namespace g1nn
+
+using namespace g1nn;
+
+extern "C" int g1_nn_rms_norm(int type, long M, int K, const void* x, long xs, const void* r, long rs, const void* w,
+                              float eps, void* y, void* h, float* rstd, void* stream) {
+  return forward<false>(type, M, K, x, xs, r, rs, w, eps, y, h, rstd, (hipStream_t)stream);
+}
+
+extern "C" int g1_nn_rms_norm_q8(int type, long M, int K, const void* x, long xs, const void* r, long rs, const void* w,
+                                 float eps, signed char* q, float* scale, void* h, void* stream) {
+  return forward<true>(type, M, K, x, xs, r, rs, w, eps, q, h, scale, (hipStream_t)stream);
+}
+
+extern "C" long g1_nn_rms_norm_backward_workspace(int type, long M, int K) {
+  (void)type;
+  return (M < kGradGrid ? M : kGradGrid) * K * (long)sizeof(float);
+}
+
+extern "C" int g1_nn_rms_norm_backward(int type, long M, int K, const void* dy, long dys, const void* dh, long dhs,
+                                       const void* h, long hs, const float* rstd, const void* w, void* dx, void* dw,
+                                       void* ws, void* stream) {
+  const hipStream_t st = (hipStream_t)stream;
+  if (bad_shape(type, M, K)) return -1;
+  long grid = 0;
+  if (M > 0) {
+    if (!dy || !h || !rstd || !w || !dx || (dw && !ws)) return refuse("a null pointer") ? -1 : 0;
+    if (bad_rows(dy, type) || bad_rows(dh, type) || bad_rows(h, type) || bad_rows(w, type) || bad_rows(dx, type) ||
+        bad_rows(dw, type))
+      return -1;
+    const NormGradArgs a{M, K, dy, dh, h, w, dys, dhs, hs, rstd, dx, dw ? (float*)ws : nullptr};
+    const bool wide = K % (type == 0 ? 4 : 8) == 0 && fits(type, K, dy, dys) && fits(type, K, dh, dhs) &&
+                      fits(type, K, h, hs) && fits(type, K, w, K) && fits(type, K, dx, K);
+    const int rc = by_type(type, wide, K, Backward{a, st, &grid});
+    if (rc) return rc;
+  }
+  if (!dw) return 0;
+  const dim3 g((K + 31) / 32);
+  if (type == 0) return launch(k_column_join<float>, g, dim3(256), st, (const float*)ws, (int)grid, K, (float*)dw);
+  return launch(k_column_join<bf16>, g, dim3(256), st, (const float*)ws, (int)grid, K, (bf16*)dw);
+}

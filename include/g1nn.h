@@ -1,0 +1,75 @@
+/* g1nn.h -- C ABI of the trainable policy's operators in libg1env.so (MI355X, gfx950): the root-mean-square
+ * norm of a residual stream (with its gradients, or with rows in 8 bits), the gated block (both projections,
+ * activation and product; with its gradients, or on 8-bit rows and weights), and the clipping of the global
+ * gradient norm. None of it has a counterpart in the reference, whose policy is a plain MLP.
+ *
+ * All pointers are DEVICE unless marked HOST. Tensors are rows of contiguous elements; where a row stride is
+ * taken it counts elements and may be zero (every row the same) or larger than the row. `type` is 0 = fp32,
+ * 1 = bf16. Sums, statistics and activations are held in 32 bits or more.
+ * Every call is asynchronous on `stream` (a hipStream_t; NULL is the null stream) of the current device, allocates
+ * nothing, keeps nothing between calls, and may be captured into a HIP graph. Workspaces are the caller's: their sizes
+ * come from the functions beside the calls, and they need 16-byte alignment.
+ * Returns 0; -1 for an argument that is refused (message on stderr, nothing enqueued); -2 for a HIP error (message on
+ * stderr).
+ */
+#ifndef G1NN_H
+#define G1NN_H
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* h = x + r (r NULL: h = x); rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * w, for M rows of K <= 32768.
+ * x and r have row strides xs and rs; w [K]; y, h [M][K] (h only where r is given, else NULL); rstd [M] fp32 or NULL.
+ * The norm is taken of the sum before it is rounded to h's type. M = 0 does nothing. */
+int g1_nn_rms_norm(int type, long M, int K, const void* x, long xs, const void* r, long rs, const void* w, float eps,
+                   void* y, void* h, float* rstd, void* stream);
+
+/* The same norm with its rows in 8 bits: y ~ q * scale, q int8 [M][K] in -127..127, scale fp32 [M] =
+ * max|y| / 127 of the row. q rounds h * w * (127 / max|h * w|) half to even: the row's norm factor cancels out of it.
+ * A row of zeros has q = 0 and scale 0 (so has one whose max|h * w| is under 4e-37); a row with an infinity or a NaN
+ * has q = 0 and scale NaN. */
+int g1_nn_rms_norm_q8(int type, long M, int K, const void* x, long xs, const void* r, long rs, const void* w, float eps,
+                      signed char* q, float* scale, void* h, void* stream);
+
+/* Gradients of g1_nn_rms_norm: from dy [M][K] (row stride dys) and, where the stream h has a gradient of its own, dh
+ * (row stride dhs; else NULL): dx [M][K], which is the gradient of x and of r alike, and dw [K] (NULL: not wanted).
+ * h (row stride hs) is the stream that the forward call wrote, or its x where there was no r. ws: a workspace of
+ * g1_nn_rms_norm_backward_workspace bytes (0 where dw is not wanted). M = 0 clears dw. */
+int g1_nn_rms_norm_backward(int type, long M, int K, const void* dy, long dys, const void* dh, long dhs, const void* h,
+                            long hs, const float* rstd, const void* w, void* dx, void* dw, void* ws, void* stream);
+long g1_nn_rms_norm_backward_workspace(int type, long M, int K);
+
+/* y = act(x Wg^T + bg) * (x Wu^T + bu): x [M][K] (row stride xs), Wg and Wu [F][K] (row strides wgs, wus), bg and bu [F]
+ * (either may be NULL), y [M][F]. act: 0 = SiLU, 1 = GELU (tanh form), 2 = sigmoid, 3 = ELU. One launch. */
+int g1_nn_gated(int type, long M, int K, int F, const void* x, long xs, const void* wg, long wgs, const void* wu,
+                long wus, const void* bg, const void* bu, int act, void* y, void* stream);
+
+/* Its gradients from dy [M][F] (row stride dys): dx [M][K], dwg and dwu [F][K], dbg and dbu [F]; any of them may be
+ * NULL (not wanted). The projections are computed again. ws: g1_nn_gated_backward_workspace bytes.
+ * M = 0 clears the gradients of the weights. */
+int g1_nn_gated_backward(int type, long M, int K, int F, const void* x, long xs, const void* wg, long wgs,
+                         const void* wu, long wus, const void* bg, const void* bu, int act, const void* dy, long dys,
+                         void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* ws, void* stream);
+long g1_nn_gated_backward_workspace(int type, long M, int K, int F);
+
+/* The gated block on 8-bit rows and weights: q [M][K] int8 (row stride qs) with scale s [M] per row, qg and qu [F][K]
+ * int8 (contiguous rows of K) with scales sg and su [F]; bg and bu fp32 [F] or NULL; y [M][F] of type `type`. The
+ * products' sums are whole numbers in 32 bits, so K <= 131072. */
+int g1_nn_gated_q8(int type, long M, int K, int F, const signed char* q, long qs, const float* s, const signed char* qg,
+                   const float* sg, const signed char* qu, const float* su, const float* bg, const float* bu, int act,
+                   void* y, void* stream);
+
+/* The global norm of n tensors (HOST arrays of n: in DEVICE pointers, in_type, out DEVICE pointers, out_type, size in
+ * elements; the tensors contiguous and aligned to their elements): norm [1] fp32 = sqrt(sum of all squares), held in 64
+ * bits until then, and out = in * min(1, max_norm / (norm + 1e-6)). out may be in (same pointer and type); then
+ * nothing is written where the factor is 1. An infinity or a NaN makes the norm one, and the factor 0 or NaN. ws:
+ * g1_nn_clip_workspace(n) bytes. n = 0 writes a norm of 0. The result does not depend on the order in which blocks run. */
+int g1_nn_clip(int n, const void* const* in, const int* in_type, void* const* out, const int* out_type,
+               const long* size, float max_norm, float* norm, void* ws, void* stream);
+long g1_nn_clip_workspace(int n);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* G1NN_H */
