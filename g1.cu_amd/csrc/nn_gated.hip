@@ -17,23 +17,33 @@ namespace g1nn {
 
 constexpr int kActs = 4;
 
-// act(g), and act'(g) where it is asked for
+// 1 / (1 + e^-x) with the hardware's exp2 and reciprocal: off by a few units in the last place of 1 + |x|
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
+
+// act(g), and act'(g) where it is asked for. GELU in its tanh form is g sigmoid(2 z), z = sqrt(2/pi) (g + 0.044715 g^3).
 template <bool D>
 __device__ __forceinline__ float activation(int act, float g, float& d) {
-  if (act == 0 || act == 2) {
-    const float p = 1.0f / (1.0f + expf(-g));
-    if (act == 2) {
-      if (D) d = p * (1.0f - p);
-      return p;
-    }
-    if (D) d = p * (1.0f + g * (1.0f - p));
+  if (act == 0) {
+    const float p = sigmoid(g);
+    if (D) d = p * __builtin_fmaf(g, 1.0f - p, 1.0f);
     return g * p;
   }
   if (act == 1) {
-    // 0.5 g (1 + tanh z) with z = sqrt(2/pi) (g + 0.044715 g^3)
-    const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g), t = tanhf(z);
-    if (D) d = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.7978845608028654f * (1.0f + 0.134145f * g * g);
-    return 0.5f * g * (1.0f + t);
+    // p is 0 or 1 long before 20, and beyond it a square or a cube could leave the range
+    const float c = __builtin_amdgcn_fmed3f(g, -20.0f, 20.0f), c2 = c * c;
+    const float p = sigmoid(1.5957691216057308f * c * __builtin_fmaf(0.044715f, c2, 1.0f));
+    if (D) {
+      d = p * __builtin_fmaf(c * (1.0f - p), 1.5957691216057308f * __builtin_fmaf(0.134145f, c2, 1.0f), 1.0f);
+      d = __builtin_fmaf(0.0f, g, d);   // a NaN stays one
+    }
+    return g * p;
+  }
+  if (act == 2) {
+    const float p = sigmoid(g);
+    if (D) d = p * (1.0f - p);
+    return p;
   }
   const float e = g > 0 ? g : expm1f(g);
   if (D) d = g > 0 ? 1.0f : e + 1.0f;
@@ -61,88 +71,100 @@ struct GatedArgs {
 using Large = Shape<128, 128, 2, 2>;
 using Small = Shape<64, 64, 2, 1>;
 
-// y, or d and its column sums
-template <typename T, typename O, typename S, bool WIDE, bool GRAD>
-__global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
-  __shared__ __align__(16) char lds[kLdsBytes<T, S>];
-  const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
-  int m, n;
-  if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
-  const Along<T> A{(const T*)a.x, a.xs, m * S::BM, a.M};
-  const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, n * (S::BN / 2), a.F};
-  typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, 0, a.K, lds, acc);
-  const int lane = threadIdx.x & 63;
+// The outputs of a block: y, or d and its column sums. FULL: the tile lies within the outputs.
+template <typename T, typename O, typename S, bool GRAD, bool FULL, int ACT>
+__device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, const typename Form<T>::Acc (&acc)[S::IM][S::JN]) {
+  const int lane = threadIdx.x & 63, rows = a.M - m * S::BM;
+  // addresses in 32 bits from the tile's first row, which is the same for all lanes
+  O* y = GRAD ? nullptr : (O*)a.y + (long)m * S::BM * a.F;
+  T* to = GRAD ? (T*)a.d + (long)m * S::BM * (2 * a.half) : nullptr;
 #pragma unroll
   for (int j = 0; j < S::JN; j += 2) {
-    const int col = c_col<S>(j), f = B.f0 + (col >> 6) * 32 + (lane & 31);
-    const bool in = f < a.F;
+    const int f = f0 + (c_col<S>(j) >> 6) * 32 + (lane & 31);
+    const bool in = FULL || f < a.F;
+    const int fc = in ? f : 0;
     float bg = 0, bu = 0, sg = 0, su = 0;
     if constexpr (sizeof(T) == 1) {
-      if (in) {
-        bg = a.bg ? ((const float*)a.bg)[f] : 0;
-        bu = a.bu ? ((const float*)a.bu)[f] : 0;
-        sg = a.sg[f];
-        su = a.su[f];
-      }
-    } else if (in) {
-      bg = a.bg ? (float)((const T*)a.bg)[f] : 0;
-      bu = a.bu ? (float)((const T*)a.bu)[f] : 0;
+      bg = a.bg ? ((const float*)a.bg)[fc] : 0;
+      bu = a.bu ? ((const float*)a.bu)[fc] : 0;
+      sg = a.sg[fc];
+      su = a.su[fc];
+    } else {
+      bg = a.bg ? (float)((const T*)a.bg)[fc] : 0;
+      bu = a.bu ? (float)((const T*)a.bu)[fc] : 0;
     }
     float sum_g = 0, sum_u = 0;
 #pragma unroll
-    for (int i = 0; i < S::IM; i++)
+    for (int i = 0; i < S::IM; i++) {
+      // what each row brings, read for sixteen rows at once
+      float given[16];
+      if constexpr (GRAD || sizeof(T) == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          int row = c_row<S>(i, r);
+          if (!FULL) row = row < rows ? row : rows - 1;
+          const long at = (long)m * S::BM + row;
+          if constexpr (GRAD) given[r] = (float)((const T*)a.dy)[at * a.dys + fc];
+          else given[r] = a.s[at];
+        }
+      }
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int tr = c_row<S>(i, r), row = m * S::BM + tr;
-        if (row >= a.M) continue;
+        const int row = c_row<S>(i, r);
         float g, u;
         if constexpr (sizeof(T) == 1) {
-          const float s = a.s[row];
-          g = (float)acc[i][j][r] * (s * sg) + bg;
-          u = (float)acc[i][j + 1][r] * (s * su) + bu;
+          g = (float)acc[i][j][r] * (given[r] * sg) + bg;
+          u = (float)acc[i][j + 1][r] * (given[r] * su) + bu;
         } else {
-          g = acc[i][j][r];
-          u = acc[i][j + 1][r];
-          if (sizeof(T) == 4 && in) {
-            if (!is_finite(g)) g = again(A, tr, B, col, 0, a.K);
-            if (!is_finite(u)) u = again(A, tr, B, col + 32, 0, a.K);
-          }
-          g += bg;
-          u += bu;
+          g = acc[i][j][r] + bg;
+          u = acc[i][j + 1][r] + bu;
         }
         float d;
-        const float v = activation<GRAD>(a.act, g, d);
+        const float v = activation<GRAD>(ACT, g, d);
+        const bool there = FULL || row < rows;
         if constexpr (!GRAD) {
-          if (in) ((O*)a.y)[(long)row * a.F + f] = (O)(v * u);
+          if (there && in) y[(unsigned)row * (unsigned)a.F + f] = (O)(v * u);
         } else {
-          float dg = 0, du = 0;
-          if (in) {
-            const float dy = (float)((const T*)a.dy)[(long)row * a.dys + f];
-            dg = dy * u * d;
-            du = dy * v;
-          }
-          T* to = (T*)a.d + (long)row * (2 * a.half);
-          if (f < a.half) {
-            to[f] = (T)dg;
-            to[a.half + f] = (T)du;
+          const float dg = there && in ? given[r] * u * d : 0, du = there && in ? given[r] * v : 0;
+          const unsigned at = (unsigned)row * (2 * a.half) + f;
+          if (there) {   // the columns from F to `half` are zeros
+            to[at] = (T)dg;
+            to[at + a.half] = (T)du;
           }
           sum_g += dg;
           sum_u += du;
         }
       }
+    }
     if constexpr (GRAD) {
       if (a.sums) {
         sum_g += __shfl_xor(sum_g, 32);
         sum_u += __shfl_xor(sum_u, 32);
-        float* to = a.sums + ((long)m * S::WM + (threadIdx.x >> 6) / S::WN) * (2 * a.half);
-        if (lane < 32 && f < a.half) {
-          to[f] = sum_g;
-          to[a.half + f] = sum_u;
+        float* at = a.sums + ((long)m * S::WM + (threadIdx.x >> 6) / S::WN) * (2 * a.half) + f;
+        if (lane < 32) {
+          at[0] = sum_g;
+          at[a.half] = sum_u;
         }
       }
     }
   }
+}
+
+template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
+__global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
+  __shared__ __align__(16) char lds[kLdsBytes<T, S>];
+  const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
+  int m, n;
+  if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
+  const int f0 = n * (S::BN / 2);
+  const Along<T> A{(const T*)a.x, a.xs, m * S::BM, a.M};
+  const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, f0, a.F};
+  typename Form<T>::Acc acc[S::IM][S::JN] = {};
+  multiply<T, S, WIDE>(A, B, 0, a.K, lds, acc);
+  if constexpr (sizeof(T) == 4)
+    mend<S>(A, B, 0, a.K, a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; }, acc);
+  if (m * S::BM + S::BM <= a.M && f0 + S::BN / 2 <= a.F) gated_out<T, O, S, GRAD, true, ACT>(a, m, f0, acc);
+  else gated_out<T, O, S, GRAD, false, ACT>(a, m, f0, acc);
 }
 
 // dx = d [Wg; Wu]
@@ -156,17 +178,17 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
   const AcrossPair<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, a.half, a.F, n * S::BN, a.K};
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
   multiply<T, S, WIDE>(A, B, 0, 2 * a.half, lds, acc);
+  const int rows = a.M - m * S::BM, cols = a.K - n * S::BN;
+  if constexpr (sizeof(T) == 4) mend<S>(A, B, 0, 2 * a.half, rows, [&](int c) { return c < cols; }, acc);
+  T* to = (T*)a.dx + (long)m * S::BM * a.K + n * S::BN;
 #pragma unroll
   for (int j = 0; j < S::JN; j++)
 #pragma unroll
     for (int i = 0; i < S::IM; i++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int tr = c_row<S>(i, r), row = m * S::BM + tr, tc = c_col<S>(j), col = n * S::BN + tc;
-        if (row >= a.M || col >= a.K) continue;
-        float v = acc[i][j][r];
-        if (sizeof(T) == 4 && !is_finite(v)) v = again(A, tr, B, tc, 0, 2 * a.half);
-        ((T*)a.dx)[(long)row * a.K + col] = (T)v;
+        const int row = c_row<S>(i, r), col = c_col<S>(j);
+        if (row < rows && col < cols) to[(unsigned)row * (unsigned)a.K + col] = (T)acc[i][j][r];
       }
 }
 
@@ -184,48 +206,53 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
   const long k0 = (long)split * a.chunk, end = k0 + a.chunk < a.M ? k0 + a.chunk : a.M;
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
   multiply<T, S, WIDE>(A, B, k0, end, lds, acc);
-  float* to = a.parts + (long)split * (2 * a.half) * a.K;
+  const int rows = 2 * a.half - m * S::BM, cols = a.K - n * S::BN;
+  if constexpr (sizeof(T) == 4) mend<S>(A, B, k0, end, rows, [&](int c) { return c < cols; }, acc);
+  float* to = a.parts + ((long)split * (2 * a.half) + m * S::BM) * a.K + n * S::BN;
 #pragma unroll
   for (int j = 0; j < S::JN; j++)
 #pragma unroll
     for (int i = 0; i < S::IM; i++)
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const int tr = c_row<S>(i, r), row = m * S::BM + tr, tc = c_col<S>(j), col = n * S::BN + tc;
-        if (row >= 2 * a.half || col >= a.K) continue;
-        float v = acc[i][j][r];
-        if (sizeof(T) == 4 && !is_finite(v)) v = again(A, tr, B, tc, k0, end);
-        to[(long)row * a.K + col] = v;
+        const int row = c_row<S>(i, r), col = c_col<S>(j);
+        if (row < rows && col < cols) to[(unsigned)row * (unsigned)a.K + col] = acc[i][j][r];
       }
 }
 
-// The parts joined: blocks [0, wide) take 256 weights each, the others 32 biases each.
+// The parts joined: blocks [0, wide) take 1024 weights each, the others 16 biases each, 64 lanes to the rows of sums.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_join(GatedArgs a, int wide) {
+__global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, int wide) {
   if ((int)blockIdx.x < wide) {
-    const long n = (long)a.F * a.K, i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long n = (long)a.F * a.K, i = (long)blockIdx.x * 1024 + threadIdx.x;
     if (i >= 2 * n) return;
     const bool up = i >= n;
-    const long at = up ? i - n : i, from = at + (up ? (long)a.half * a.K : 0), step = 2l * a.half * a.K;
+    const long at = up ? i - n : i, step = 2l * a.half * a.K;
+    const float* from = a.parts + at + (up ? (long)a.half * a.K : 0);
     T* to = (T*)(up ? a.dwu : a.dwg);
     if (!to) return;
     float v = 0;
-    for (int s = 0; s < a.splits; s++) v += a.parts[s * step + from];
+#pragma unroll 4
+    for (int s = 0; s < a.splits; s++) v += from[s * step];
     to[at] = (T)v;
     return;
   }
-  __shared__ float part[8][32];
-  const int c = threadIdx.x & 31, o = threadIdx.x >> 5, i = (blockIdx.x - wide) * 32 + c;
+  __shared__ float part[64][17];
+  const int c = threadIdx.x & 15, o = threadIdx.x >> 4, i = (blockIdx.x - wide) * 16 + c;
   const bool up = i >= a.half;
   const int f = up ? i - a.half : i;
   T* to = (T*)(up ? a.dbu : a.dbg);
   float v = 0;
-  if (to && f < a.F)
-    for (int p = o; p < a.sum_rows; p += 8) v += a.sums[(long)p * (2 * a.half) + i];
+  if (to && f < a.F) {
+    const float* from = a.sums + i;
+    const long step = 2l * a.half;
+#pragma unroll 8
+    for (int p = o; p < a.sum_rows; p += 64) v += from[p * step];
+  }
   part[o][c] = v;
   __syncthreads();
   if (o == 0 && to && f < a.F) {
-    for (int p = 1; p < 8; p++) v += part[p][c];
+    for (int p = 1; p < 64; p++) v += part[p][c];
     to[f] = (T)v;
   }
 }
@@ -234,17 +261,27 @@ __global__ __launch_bounds__(256) void k_gated_join(GatedArgs a, int wide) {
 // Tiles of 128 x 128 where they give every CU one; else of 64 x 64, four times as many.
 inline bool large(long m, long n) { return ((m + 127) / 128) * ((n + 127) / 128) >= 256; }
 
-template <typename T, typename O, typename S, bool GRAD>
+template <typename T, typename O, typename S, bool GRAD, int ACT>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
   const dim3 grid(tile_grid((a.M + S::BM - 1) / S::BM, ((GRAD ? a.half : a.F) + S::BN / 2 - 1) / (S::BN / 2)));
-  if (wide) return launch(k_gated<T, O, S, true, GRAD>, grid, dim3(S::kThreads), st, a);
-  return launch(k_gated<T, O, S, false, GRAD>, grid, dim3(S::kThreads), st, a);
+  if (wide) return launch(k_gated<T, O, S, true, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
+  return launch(k_gated<T, O, S, false, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
+}
+
+template <typename T, typename O, bool GRAD, int ACT>
+int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
+  if (large(a.M, 2l * a.F)) return run_gated<T, O, Large, GRAD, ACT>(a, wide, st);
+  return run_gated<T, O, Small, GRAD, ACT>(a, wide, st);
 }
 
 template <typename T, typename O, bool GRAD>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
-  if (large(a.M, 2l * a.F)) return run_gated<T, O, Large, GRAD>(a, wide, st);
-  return run_gated<T, O, Small, GRAD>(a, wide, st);
+  switch (a.act) {
+    case 0: return run_gated<T, O, GRAD, 0>(a, wide, st);
+    case 1: return run_gated<T, O, GRAD, 1>(a, wide, st);
+    case 2: return run_gated<T, O, GRAD, 2>(a, wide, st);
+    default: return run_gated<T, O, GRAD, 3>(a, wide, st);
+  }
 }
 
 template <typename T, typename S>
@@ -306,9 +343,9 @@ inline bool bad_place(int type, std::initializer_list<const void*> ps) {
   return false;
 }
 
-// Whether rows of n elements can be read in accesses of `bytes`.
+// Whether rows of n elements can be read in accesses of `bytes`, a tile of them with 32-bit offsets.
 inline bool even(const void* p, long stride, long n, int size, int bytes) {
-  return aligned(p, bytes) && stride * size % bytes == 0 && n * size % bytes == 0;
+  return aligned(p, bytes) && stride * size % bytes == 0 && n * size % bytes == 0 && stride <= (1 << 22);
 }
 
 template <typename T>
@@ -335,8 +372,8 @@ int gated_backward(GatedArgs a, const Split& s, hipStream_t st) {
     a.splits = a.sum_rows = 0;
   }
   if (!weights && !biases) return 0;
-  const long nw = weights ? (2l * a.F * a.K + 255) / 256 : 0, nb = biases ? 2 * a.half / 32 : 0;
-  return launch(k_gated_join<T>, dim3((unsigned)(nw + nb)), dim3(256), st, a, (int)nw);
+  const long nw = weights ? (2l * a.F * a.K + 1023) / 1024 : 0, nb = biases ? 2 * a.half / 16 : 0;
+  return launch(k_gated_join<T>, dim3((unsigned)(nw + nb)), dim3(1024), st, a, (int)nw);
 }
 
 }  // namespace g1nn

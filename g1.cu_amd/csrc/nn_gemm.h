@@ -18,8 +18,10 @@
 namespace g1nn {
 
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -55,14 +57,20 @@ __device__ __forceinline__ int lds_at(int rows, int plane, int row, int c) {
   return ((plane * rows + row) * kSlots<T> + (c ^ s)) * 16;
 }
 
-// x = hi + mid + lo, each rounded to nearest
-template <typename F, typename B>
-__device__ __forceinline__ void split(F x, B& hi, B& mid, B& lo) {
-  hi = __builtin_convertvector(x, B);
-  x -= __builtin_convertvector(hi, F);
-  mid = __builtin_convertvector(x, B);
-  x -= __builtin_convertvector(mid, F);
-  lo = __builtin_convertvector(x, B);
+// N values as N/2 words of two bf16 numbers each, x = hi + mid + lo, each rounded to nearest: 11 operations a pair.
+template <int N>
+__device__ __forceinline__ void split(const float (&x)[N], unsigned (&hi)[N / 2], unsigned (&mid)[N / 2], unsigned (&lo)[N / 2]) {
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) {
+    f32x2 v = {x[2 * i], x[2 * i + 1]};
+    hi[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+    v[0] -= __uint_as_float(hi[i] << 16);
+    v[1] -= __uint_as_float(hi[i] & 0xffff0000u);
+    mid[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+    v[0] -= __uint_as_float(mid[i] << 16);
+    v[1] -= __uint_as_float(mid[i] & 0xffff0000u);
+    lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+  }
 }
 
 // ---- operands: where the rows of a tile lie ---------------------------------------------------------------------
@@ -96,20 +104,23 @@ struct Paired {
   __device__ T at(int r, int k) const { return row(r)[k]; }
 };
 
-// Across: k counts the rows of memory, and the tile's rows are its columns [col0, cols). line(k) is the start of
-// memory row k.
+// Across: k counts the rows of memory, and the tile's rows are its columns [col0, cols). tile(k0) is the start of the
+// memory row k0, from which the tile's rows follow `step(k0)` apart, and whole(k0, n) says whether all n exist.
 template <typename T>
 struct Across {
   static constexpr bool kAlong = false;
   const T* p;
   long stride;
   int col0, cols;
-  __device__ const T* line(long k) const { return p + k * stride; }
+  __device__ const T* tile(long k0) const { return p + k0 * stride; }
+  __device__ long step(long) const { return stride; }
+  __device__ bool whole(long, int) const { return true; }
   __device__ bool has(long) const { return true; }
-  __device__ T at(int r, long k) const { return line(k)[col0 + r < cols ? col0 + r : cols - 1]; }
+  __device__ T at(int r, long k) const { return p[k * stride + col0 + r]; }
 };
 
-// Across the rows of both weights one after the other, each padded to `half` rows of which F exist.
+// Across the rows of both weights one after the other, each padded to `half` rows (a multiple of every tile's depth) of
+// which F exist.
 template <typename T>
 struct AcrossPair {
   static constexpr bool kAlong = false;
@@ -117,9 +128,11 @@ struct AcrossPair {
   long gs, us;
   int half, F;
   int col0, cols;
-  __device__ const T* line(long k) const { return k < half ? g + k * gs : u + (k - half) * us; }
+  __device__ const T* tile(long k0) const { return k0 < half ? g + k0 * gs : u + (k0 - half) * us; }
+  __device__ long step(long k0) const { return k0 < half ? gs : us; }
+  __device__ bool whole(long k0, int n) const { return (k0 < half ? k0 : k0 - half) + n <= F; }
   __device__ bool has(long k) const { return (k < half ? k : k - half) < F; }
-  __device__ T at(int r, long k) const { return has(k) ? line(k)[col0 + r < cols ? col0 + r : cols - 1] : (T)0.0f; }
+  __device__ T at(int r, long k) const { return has(k) ? tile(k)[col0 + r] : (T)0.0f; }
 };
 
 // ---- staging: global memory -> registers -> LDS -----------------------------------------------------------------
@@ -147,6 +160,13 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
     }
   }
   __device__ __forceinline__ void load(const Op&, long k0, long end) {
+    if (WIDE && k0 + kDepth<T> <= end) {
+#pragma unroll
+      for (int i = 0; i < kUnits; i++)
+#pragma unroll
+        for (int a = 0; a < kAcc; a++) v[i].w[a] = reinterpret_cast<const i32x4*>(at[i] + k0)[a];
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       const T* p = at[i] + k0;
@@ -166,13 +186,11 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
     for (int i = 0; i < kUnits; i++) {
       const int u = threadIdx.x + i * THREADS, row = u / kSlots<T>, c = u % kSlots<T>;
       if constexpr (sizeof(T) == 4) {
-        f32x8 x;
+        unsigned h[3][4];
+        split(v[i].e, h[0], h[1], h[2]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = v[i].e[e];
-        bf16x8 h[3];
-        split(x, h[0], h[1], h[2]);
-#pragma unroll
-        for (int p = 0; p < 3; p++) *reinterpret_cast<bf16x8*>(lds + lds_at<T>(ROWS, p, row, c)) = h[p];
+        for (int p = 0; p < 3; p++)
+          *reinterpret_cast<u32x4*>(lds + lds_at<T>(ROWS, p, row, c)) = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
       } else {
         *reinterpret_cast<i32x4*>(lds + lds_at<T>(ROWS, 0, row, c)) = v[i].w[0];
       }
@@ -188,29 +206,33 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
   static_assert(kQuads * (kDepth<T> / kLines) % THREADS == 0, "whole units");
   typedef T Quad __attribute__((ext_vector_type(4)));
   Quad v[kUnits][kLines];
-  int col[kUnits];
 
-  __device__ __forceinline__ void init(const Op& o) {
-#pragma unroll
-    for (int i = 0; i < kUnits; i++) {
-      const int c = o.col0 + (threadIdx.x + i * THREADS) % kQuads * 4;
-      col[i] = WIDE ? (c < o.cols ? c : 0) : c;   // past the end: any column, whose values go nowhere
-    }
-  }
+  __device__ __forceinline__ void init(const Op&) {}
   __device__ __forceinline__ void load(const Op& o, long k0, long end) {
+    const T* p = o.tile(k0);
+    const long step = o.step(k0);
+    if (WIDE && k0 + kDepth<T> <= end && o.whole(k0, kDepth<T>)) {
+      // offsets from a common start, in 32 bits: the host takes strides up to 2^22 elements
+#pragma unroll
+      for (int i = 0; i < kUnits; i++) {
+        const int u = threadIdx.x + i * THREADS, c = o.col0 + u % kQuads * 4;
+        // columns past the end: any one, whose values go nowhere
+        const unsigned at = (unsigned)(u / kQuads * kLines) * (unsigned)step + (unsigned)(c < o.cols ? c : 0);
+#pragma unroll
+        for (int l = 0; l < kLines; l++) v[i][l] = *reinterpret_cast<const Quad*>(p + l * step + at);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const long k = k0 + (threadIdx.x + i * THREADS) / kQuads * kLines;
+      const int u = threadIdx.x + i * THREADS, c = o.col0 + u % kQuads * 4;
 #pragma unroll
       for (int l = 0; l < kLines; l++) {
-        const bool ok = k + l < end && o.has(k + l);
-        if (WIDE) {
-          if (ok) v[i][l] = *reinterpret_cast<const Quad*>(o.line(k + l) + col[i]);
-          else v[i][l] = Quad{0, 0, 0, 0};
-        } else {
+        const int k = u / kQuads * kLines + l;
+        const bool ok = k0 + k < end && o.has(k0 + k);
+        const T* q = p + k * step + c;
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[i][l][e] = ok && col[i] + e < o.cols ? o.line(k + l)[col[i] + e] : (T)0;
-        }
+        for (int e = 0; e < 4; e++) v[i][l][e] = ok && c + e < o.cols ? q[e] : (T)0.0f;
       }
     }
   }
@@ -221,12 +243,12 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         if constexpr (sizeof(T) == 4) {
-          const f32x4 x = {v[i][0][e], v[i][1][e], v[i][2][e], v[i][3][e]};
-          bf16x4 h[3];
+          const float x[4] = {v[i][0][e], v[i][1][e], v[i][2][e], v[i][3][e]};
+          unsigned h[3][2];
           split(x, h[0], h[1], h[2]);
 #pragma unroll
           for (int p = 0; p < 3; p++)
-            *reinterpret_cast<bf16x4*>(lds + lds_at<T>(ROWS, p, row + e, part >> 1) + (part & 1) * 8) = h[p];
+            *reinterpret_cast<u32x2*>(lds + lds_at<T>(ROWS, p, row + e, part >> 1) + (part & 1) * 8) = u32x2{h[p][0], h[p][1]};
         } else {
           bf16x8 h;
 #pragma unroll
@@ -327,8 +349,6 @@ __device__ __attribute__((noinline)) float again(const OpA& A, int ra, const OpB
   return v;
 }
 
-__device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-
 // row of C (within the block's tile) that register r of accumulator i holds
 template <typename S>
 __device__ __forceinline__ int c_row(int i, int r) {
@@ -339,6 +359,30 @@ __device__ __forceinline__ int c_row(int i, int r) {
 template <typename S>
 __device__ __forceinline__ int c_col(int j) {
   return (int)(threadIdx.x >> 6) % S::WN * S::JN * 32 + j * 32 + (threadIdx.x & 31);
+}
+
+// The fp32 outputs that came out infinite or NaN, again: those of rows below `rows` and of columns that are stored
+// (a column is one of them where stored(column)).
+template <typename S, typename OpA, typename OpB, typename C>
+__device__ __forceinline__ void mend(const OpA& A, const OpB& B, long k0, long end, int rows, C stored,
+                                     f32x16 (&acc)[S::IM][S::JN]) {
+  float z = 0;   // stays zero unless one of them is: a multiplication each
+#pragma unroll
+  for (int i = 0; i < S::IM; i++)
+#pragma unroll
+    for (int j = 0; j < S::JN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) z = __builtin_fmaf(acc[i][j][r], 0.0f, z);
+  if (z == 0) return;
+#pragma unroll
+  for (int i = 0; i < S::IM; i++)
+#pragma unroll
+    for (int j = 0; j < S::JN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int row = c_row<S>(i, r), col = c_col<S>(j);
+        if (acc[i][j][r] * 0.0f != 0 && row < rows && stored(col)) acc[i][j][r] = again(A, row, B, col, k0, end);
+      }
 }
 
 // Blocks to tiles (rows of tiles `tm`, `tn` in each): block b runs on XCD b mod 8, and a row of tiles stays on one
