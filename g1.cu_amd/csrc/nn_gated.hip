@@ -152,7 +152,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
 
 template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
 __global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
-  __shared__ __align__(16) char lds[kLdsBytes<T, S>];
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
   const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
   int m, n;
   if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
@@ -160,9 +160,10 @@ __global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
   const Along<T> A{(const T*)a.x, a.xs, m * S::BM, a.M};
   const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, f0, a.F};
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, 0, a.K, lds, acc);
+  multiply<T, S, WIDE>(A, B, 0, a.K, lds0, lds1, acc);
   if constexpr (sizeof(T) == 4)
-    mend<S>(A, B, 0, a.K, a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; }, acc);
+    mend<S>(a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; },
+            [&](int r, int c) { return again(A, r, B, c, 0, a.K); }, acc);
   if (m * S::BM + S::BM <= a.M && f0 + S::BN / 2 <= a.F) gated_out<T, O, S, GRAD, true, ACT>(a, m, f0, acc);
   else gated_out<T, O, S, GRAD, false, ACT>(a, m, f0, acc);
 }
@@ -170,16 +171,19 @@ __global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
 // dx = d [Wg; Wu]
 template <typename T, typename S, bool WIDE>
 __global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
-  __shared__ __align__(16) char lds[kLdsBytes<T, S>];
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
   const int tm = (a.M + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
   int m, n;
   if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
-  const Along<T> A{(const T*)a.d, 2l * a.half, m * S::BM, a.M};
-  const AcrossPair<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, a.half, a.F, n * S::BN, a.K};
+  const Along<T> dg{(const T*)a.d, 2l * a.half, m * S::BM, a.M}, du{dg.p + a.half, dg.stride, dg.row0, dg.rows};
+  const Across<T> wg{(const T*)a.wg, a.wgs, n * S::BN, a.K}, wu{(const T*)a.wu, a.wus, n * S::BN, a.K};
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, 0, 2 * a.half, lds, acc);
+  multiply<T, S, WIDE>(dg, wg, 0, a.F, lds0, lds1, acc);
+  multiply<T, S, WIDE>(du, wu, 0, a.F, lds0, lds1, acc);
   const int rows = a.M - m * S::BM, cols = a.K - n * S::BN;
-  if constexpr (sizeof(T) == 4) mend<S>(A, B, 0, 2 * a.half, rows, [&](int c) { return c < cols; }, acc);
+  if constexpr (sizeof(T) == 4)
+    mend<S>(rows, [&](int c) { return c < cols; },
+            [&](int r, int c) { return again(dg, r, wg, c, 0, a.F) + again(du, r, wu, c, 0, a.F); }, acc);
   T* to = (T*)a.dx + (long)m * S::BM * a.K + n * S::BN;
 #pragma unroll
   for (int j = 0; j < S::JN; j++)
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
 // then reads those rows of d and x from memory once.
 template <typename T, typename S, bool WIDE>
 __global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
-  __shared__ __align__(16) char lds[kLdsBytes<T, S>];
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
   const int tm = (2 * a.half + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
   int split, t;
   if (!tile_of(blockIdx.x, a.splits, tm * tn, split, t)) return;
@@ -205,9 +209,10 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
   const Across<T> B{(const T*)a.x, a.xs, n * S::BN, a.K};
   const long k0 = (long)split * a.chunk, end = k0 + a.chunk < a.M ? k0 + a.chunk : a.M;
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, k0, end, lds, acc);
+  multiply<T, S, WIDE>(A, B, k0, end, lds0, lds1, acc);
   const int rows = 2 * a.half - m * S::BM, cols = a.K - n * S::BN;
-  if constexpr (sizeof(T) == 4) mend<S>(A, B, k0, end, rows, [&](int c) { return c < cols; }, acc);
+  if constexpr (sizeof(T) == 4)
+    mend<S>(rows, [&](int c) { return c < cols; }, [&](int r, int c) { return again(A, r, B, c, k0, end); }, acc);
   float* to = a.parts + ((long)split * (2 * a.half) + m * S::BM) * a.K + n * S::BN;
 #pragma unroll
   for (int j = 0; j < S::JN; j++)
@@ -337,15 +342,21 @@ inline bool bad_gated(int type, long M, int K, int F, int act) {
   return false;
 }
 
+inline bool bad_strides(std::initializer_list<long> strides) {
+  for (const long s : strides)
+    if (s < 0 || s > (1l << 22)) return refuse("row strides of 0 to 2^22 elements are supported");
+  return false;
+}
+
 inline bool bad_place(int type, std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (!aligned(p, type == 0 ? 4 : 2)) return refuse("an address is not aligned to its elements");
   return false;
 }
 
-// Whether rows of n elements can be read in accesses of `bytes`, a tile of them with 32-bit offsets.
+// Whether rows of n elements can be read in accesses of `bytes`.
 inline bool even(const void* p, long stride, long n, int size, int bytes) {
-  return aligned(p, bytes) && stride * size % bytes == 0 && n * size % bytes == 0 && stride <= (1 << 22);
+  return aligned(p, bytes) && stride * size % bytes == 0 && n * size % bytes == 0;
 }
 
 template <typename T>
@@ -385,7 +396,7 @@ extern "C" int g1_nn_gated(int type, long M, int K, int F, const void* x, long x
   if (bad_gated(type, M, K, F, act)) return -1;
   if (M == 0) return 0;
   if (!x || !wg || !wu || !y) return refuse("a null pointer") ? -1 : 0;
-  if (bad_place(type, {x, wg, wu, bg, bu, y})) return -1;
+  if (bad_place(type, {x, wg, wu, bg, bu, y}) || bad_strides({xs, wgs, wus})) return -1;
   GatedArgs a{};
   a.M = (int)M, a.K = K, a.F = F, a.x = x, a.wg = wg, a.wu = wu, a.bg = bg, a.bu = bu;
   a.xs = xs, a.wgs = wgs, a.wus = wus, a.act = act, a.y = y;
@@ -405,7 +416,7 @@ extern "C" int g1_nn_gated_backward(int type, long M, int K, int F, const void* 
                                     void* stream) {
   if (bad_gated(type, M, K, F, act)) return -1;
   if (M > 0 && (!x || !wg || !wu || !dy || !ws)) return refuse("a null pointer") ? -1 : 0;
-  if (bad_place(type, {x, wg, wu, bg, bu, dy, dx, dwg, dwu, dbg, dbu})) return -1;
+  if (bad_place(type, {x, wg, wu, bg, bu, dy, dx, dwg, dwu, dbg, dbu}) || bad_strides({xs, wgs, wus, dys})) return -1;
   if (!aligned(ws, 16)) return refuse("the workspace is not aligned to 16 bytes") ? -1 : 0;
   const Split s(M, K, F);
   const Workspace w(type, M, K, s);
@@ -425,7 +436,7 @@ extern "C" int g1_nn_gated_q8(int type, long M, int K, int F, const signed char*
   if (bad_gated(type, M, K, F, act)) return -1;
   if (M == 0) return 0;
   if (!q || !s || !qg || !sg || !qu || !su || !y) return refuse("a null pointer") ? -1 : 0;
-  if (bad_place(type, {y}) || bad_place(0, {s, sg, su, bg, bu})) return -1;
+  if (bad_place(type, {y}) || bad_place(0, {s, sg, su, bg, bu}) || bad_strides({qs})) return -1;
   GatedArgs a{};
   a.M = (int)M, a.K = K, a.F = F, a.x = q, a.wg = qg, a.wu = qu, a.bg = bg, a.bu = bu;
   a.xs = qs, a.wgs = a.wus = K, a.act = act, a.y = y, a.s = s, a.sg = sg, a.su = su;

@@ -10,13 +10,16 @@
 // one, so six products beat one. Where a sum comes out infinite or NaN (an operand was, or was too large to round to
 // bf16: a rest of an infinity is NaN), that output is summed again in plain fp32, so it is what the formula gives.
 //
-// LDS. A chunk (row, c) lies in the row's slot c ^ swizzle(row): the eight rows of a phase of a 16-byte read, and the
-// rows four apart that a transposing store writes, fall into different banks.
+// LDS. A tile's row has kSlots chunks; a chunk c lies in the row's slot c ^ (some bits of the row), so that the sixteen
+// rows of a phase of a 16-byte read fall into different banks (64 of them: 256 bytes a cycle).
 #pragma once
+#include <type_traits>
+
 #include "nn_common.h"
 
 namespace g1nn {
 
+typedef signed char i8;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -25,37 +28,43 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef signed char i8;
 
-// How a type goes through the matrix cores: planes in LDS, bytes of a plane's row, elements per 16-byte chunk.
+// How a type goes through the matrix cores: planes in LDS, elements per 16-byte chunk, chunks of a row of a tile.
 template <typename T>
 struct Form;
 template <>
 struct Form<float> {
-  static constexpr int kPlanes = 3, kRowBytes = 64, kPer = 8;
+  static constexpr int kPlanes = 3, kPer = 8, kSlots = 2;
   typedef f32x16 Acc;
 };
 template <>
 struct Form<bf16> {
-  static constexpr int kPlanes = 1, kRowBytes = 128, kPer = 8;
+  static constexpr int kPlanes = 1, kPer = 8, kSlots = 8;
   typedef f32x16 Acc;
 };
 template <>
 struct Form<i8> {
-  static constexpr int kPlanes = 1, kRowBytes = 128, kPer = 16;
+  static constexpr int kPlanes = 1, kPer = 16, kSlots = 4;
   typedef i32x16 Acc;
 };
 
 template <typename T>
-constexpr int kSlots = Form<T>::kRowBytes / 16;          // chunks of a row
+constexpr int kSlots = Form<T>::kSlots;
 template <typename T>
 constexpr int kDepth = kSlots<T> * Form<T>::kPer;        // k of a tile
 
 template <typename T>
-__device__ __forceinline__ int lds_at(int rows, int plane, int row, int c) {
-  const int s = kSlots<T> == 8 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
-  return ((plane * rows + row) * kSlots<T> + (c ^ s)) * 16;
+__device__ __forceinline__ int swizzle(int row) {
+  return kSlots<T> == 2 ? (row >> 3) & 1 : kSlots<T> == 4 ? (row >> 2) & 3 : (row ^ (row >> 3)) & 7;
 }
+template <typename T>
+__device__ __forceinline__ int lds_at(int rows, int plane, int row, int c) {
+  return ((plane * rows + row) * kSlots<T> + (c ^ swizzle<T>(row))) * 16;
+}
+
+__device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ unsigned bits(bf16 v) { return __builtin_bit_cast(unsigned short, v); }
+__device__ __forceinline__ unsigned bits(i8 v) { return (unsigned char)v; }
 
 // N values as N/2 words of two bf16 numbers each, x = hi + mid + lo, each rounded to nearest: 11 operations a pair.
 template <int N>
@@ -74,19 +83,18 @@ __device__ __forceinline__ void split(const float (&x)[N], unsigned (&hi)[N / 2]
 }
 
 // ---- operands: where the rows of a tile lie ---------------------------------------------------------------------
-// Along: a row's k are contiguous. row(r) is the start of the tile's row r; rows past the end repeat the last one, and
-// what they give is never stored.
+// Along: a row's k are contiguous. Row r of the tile starts at base(r) + offset(r): a base that is the same for the 32
+// rows around r, and an offset in 32 bits (the host refuses strides over 2^22 elements). Rows past the end repeat the
+// last one, and what they give is never stored.
 template <typename T>
 struct Along {
   static constexpr bool kAlong = true;
   const T* p;
   long stride;
   int row0, rows;
-  __device__ const T* row(int r) const {
-    const int i = row0 + r;
-    return p + (long)(i < rows ? i : rows - 1) * stride;
-  }
-  __device__ T at(int r, int k) const { return row(r)[k]; }
+  __device__ const T* base(int) const { return p + (long)row0 * stride; }
+  __device__ unsigned offset(int r) const { return (unsigned)min(r, rows - row0 - 1) * (unsigned)stride; }
+  __device__ T at(int r, long k) const { return p[(row0 + (long)r) * stride + k]; }
 };
 
 // Both projections' weights in one tile: 32 rows of the gate, then the 32 of the other projection for the same
@@ -97,47 +105,29 @@ struct Paired {
   const T *g, *u;
   long gs, us;
   int f0, F;
-  __device__ const T* row(int r) const {
-    const int i = f0 + (r >> 6) * 32 + (r & 31), c = i < F ? i : F - 1;
-    return (r & 32) ? u + (long)c * us : g + (long)c * gs;
+  // a tile may begin past F (the padding of d): it repeats the last output's weights
+  __device__ const T* base(int r) const {
+    const long f = min(f0, F - 1);
+    return (r & 32) ? u + f * us : g + f * gs;
   }
-  __device__ T at(int r, int k) const { return row(r)[k]; }
+  __device__ unsigned offset(int r) const {
+    return (unsigned)max(min((r >> 6) * 32 + (r & 31), F - f0 - 1), 0) * (unsigned)((r & 32) ? us : gs);
+  }
+  __device__ T at(int r, long k) const { return base(r)[((r >> 6) * 32 + (r & 31)) * ((r & 32) ? us : gs) + k]; }
 };
 
-// Across: k counts the rows of memory, and the tile's rows are its columns [col0, cols). tile(k0) is the start of the
-// memory row k0, from which the tile's rows follow `step(k0)` apart, and whole(k0, n) says whether all n exist.
+// Across: k counts the rows of memory, and the tile's rows are its columns [col0, cols).
 template <typename T>
 struct Across {
   static constexpr bool kAlong = false;
   const T* p;
   long stride;
   int col0, cols;
-  __device__ const T* tile(long k0) const { return p + k0 * stride; }
-  __device__ long step(long) const { return stride; }
-  __device__ bool whole(long, int) const { return true; }
-  __device__ bool has(long) const { return true; }
   __device__ T at(int r, long k) const { return p[k * stride + col0 + r]; }
 };
 
-// Across the rows of both weights one after the other, each padded to `half` rows (a multiple of every tile's depth) of
-// which F exist.
-template <typename T>
-struct AcrossPair {
-  static constexpr bool kAlong = false;
-  const T *g, *u;
-  long gs, us;
-  int half, F;
-  int col0, cols;
-  __device__ const T* tile(long k0) const { return k0 < half ? g + k0 * gs : u + (k0 - half) * us; }
-  __device__ long step(long k0) const { return k0 < half ? gs : us; }
-  __device__ bool whole(long k0, int n) const { return (k0 < half ? k0 : k0 - half) + n <= F; }
-  __device__ bool has(long k) const { return (k < half ? k : k - half) < F; }
-  __device__ T at(int r, long k) const { return has(k) ? tile(k)[col0 + r] : (T)0.0f; }
-};
-
-// ---- staging: global memory -> registers -> LDS -----------------------------------------------------------------
-// WIDE: every chunk's elements lie within the operand and can be read in one aligned access (the host has checked
-// addresses, strides and lengths); otherwise they are read one by one.
+// ---- staging through registers: fp32, and rows that 16-byte accesses do not fit ------------------------------------
+// WIDE: the host has checked that every chunk's elements lie within the operand and can be read in aligned accesses.
 template <typename T, typename Op, int ROWS, int THREADS, bool WIDE, bool ALONG = Op::kAlong>
 struct Stage;
 
@@ -145,118 +135,188 @@ template <typename T, typename Op, int ROWS, int THREADS, bool WIDE>
 struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
   static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * kSlots<T> / THREADS, kAcc = sizeof(T) == 4 ? 2 : 1;
   static_assert(ROWS * kSlots<T> % THREADS == 0, "whole units");
-  union Chunk {
-    i32x4 w[kAcc];
-    T e[kPer];
-  };
-  const T* at[kUnits];
-  Chunk v[kUnits];
+  unsigned off[kUnits];
+  i32x4 v[kUnits][kAcc];
 
+  static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
+  // a wave's unit lies within 32 rows: one base
+  static __device__ __forceinline__ const T* base(const Op& o, int i) {
+    return o.base(__builtin_amdgcn_readfirstlane(unit(i) / kSlots<T>));
+  }
   __device__ __forceinline__ void init(const Op& o) {
 #pragma unroll
-    for (int i = 0; i < kUnits; i++) {
-      const int u = threadIdx.x + i * THREADS;
-      at[i] = o.row(u / kSlots<T>) + u % kSlots<T> * kPer;
-    }
+    for (int i = 0; i < kUnits; i++) off[i] = o.offset(unit(i) / kSlots<T>) + unit(i) % kSlots<T> * kPer;
   }
-  __device__ __forceinline__ void load(const Op&, long k0, long end) {
-    if (WIDE && k0 + kDepth<T> <= end) {
+  __device__ __forceinline__ void load(const Op& o, long k0) {
+    if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < kUnits; i++)
 #pragma unroll
-        for (int a = 0; a < kAcc; a++) v[i].w[a] = reinterpret_cast<const i32x4*>(at[i] + k0)[a];
-      return;
+        for (int a = 0; a < kAcc; a++) v[i][a] = reinterpret_cast<const i32x4*>(base(o, i) + k0 + off[i])[a];
+    } else {
+      load(o, k0, k0 + kDepth<T>);
     }
+  }
+  // zeros from `end`
+  __device__ __forceinline__ void load(const Op& o, long k0, long end) {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const T* p = at[i] + k0;
-      const long k = k0 + (threadIdx.x + i * THREADS) % kSlots<T> * kPer;
-      if (WIDE) {
+      const T* p = base(o, i) + k0 + off[i];
+      const int n = (int)(end - k0) - unit(i) % kSlots<T> * kPer;
+      constexpr int kIn = 4 / sizeof(T);   // elements of a word
 #pragma unroll
-        for (int a = 0; a < kAcc; a++)
-          v[i].w[a] = k + a * (16 / (int)sizeof(T)) < end ? reinterpret_cast<const i32x4*>(p)[a] : i32x4{0, 0, 0, 0};
-      } else {
+      for (int w = 0; w < kPer / kIn; w++) {
+        unsigned word = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) v[i].e[e] = k + e < end ? p[e] : (T)0;
+        for (int e = 0; e < kIn; e++)
+          if (w * kIn + e < n) word |= bits(p[w * kIn + e]) << (e * 8 * sizeof(T));
+        v[i][w / 4][w % 4] = (int)word;
       }
     }
   }
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const int u = threadIdx.x + i * THREADS, row = u / kSlots<T>, c = u % kSlots<T>;
+      const int row = unit(i) / kSlots<T>, c = unit(i) % kSlots<T>;
+      char* to = lds + lds_at<T>(ROWS, 0, row, c);
       if constexpr (sizeof(T) == 4) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __int_as_float(v[i][e / 4][e % 4]);
         unsigned h[3][4];
-        split(v[i].e, h[0], h[1], h[2]);
+        split(x, h[0], h[1], h[2]);
 #pragma unroll
         for (int p = 0; p < 3; p++)
-          *reinterpret_cast<u32x4*>(lds + lds_at<T>(ROWS, p, row, c)) = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
+          *reinterpret_cast<u32x4*>(to + p * ROWS * kSlots<T> * 16) = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
       } else {
-        *reinterpret_cast<i32x4*>(lds + lds_at<T>(ROWS, 0, row, c)) = v[i].w[0];
+        *reinterpret_cast<i32x4*>(to) = v[i][0];
       }
     }
   }
 };
 
-// Transposing: a unit is four columns of kLines consecutive memory rows (a chunk, or half of one in fp32).
+// Transposing: a unit is four consecutive memory rows (half a chunk) of two fp32 or four bf16 columns.
 template <typename T, typename Op, int ROWS, int THREADS, bool WIDE>
 struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
-  static constexpr int kLines = sizeof(T) == 4 ? 4 : 8, kQuads = ROWS / 4;
-  static constexpr int kUnits = kQuads * (kDepth<T> / kLines) / THREADS;
-  static_assert(kQuads * (kDepth<T> / kLines) % THREADS == 0, "whole units");
-  typedef T Quad __attribute__((ext_vector_type(4)));
-  Quad v[kUnits][kLines];
+  static constexpr int kCols = 8 / sizeof(T), kWidth = ROWS / kCols, kUnits = kWidth * (kDepth<T> / 4) / THREADS;
+  static_assert(kWidth * (kDepth<T> / 4) % THREADS == 0, "whole units");
+  unsigned off[kUnits];
+  u32x2 v[kUnits][4];
 
-  __device__ __forceinline__ void init(const Op&) {}
-  __device__ __forceinline__ void load(const Op& o, long k0, long end) {
-    const T* p = o.tile(k0);
-    const long step = o.step(k0);
-    if (WIDE && k0 + kDepth<T> <= end && o.whole(k0, kDepth<T>)) {
-      // offsets from a common start, in 32 bits: the host takes strides up to 2^22 elements
-#pragma unroll
-      for (int i = 0; i < kUnits; i++) {
-        const int u = threadIdx.x + i * THREADS, c = o.col0 + u % kQuads * 4;
-        // columns past the end: any one, whose values go nowhere
-        const unsigned at = (unsigned)(u / kQuads * kLines) * (unsigned)step + (unsigned)(c < o.cols ? c : 0);
-#pragma unroll
-        for (int l = 0; l < kLines; l++) v[i][l] = *reinterpret_cast<const Quad*>(p + l * step + at);
-      }
-      return;
-    }
+  static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
+  __device__ __forceinline__ void init(const Op& o) {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const int u = threadIdx.x + i * THREADS, c = o.col0 + u % kQuads * 4;
+      const int c = o.col0 + unit(i) % kWidth * kCols;
+      // columns past the end: the first ones, whose values go nowhere
+      off[i] = (unsigned)(unit(i) / kWidth * 4) * (unsigned)o.stride + (unsigned)(c < o.cols ? c : 0);
+    }
+  }
+  __device__ __forceinline__ void load(const Op& o, long k0) {
+    if constexpr (WIDE) {
 #pragma unroll
-      for (int l = 0; l < kLines; l++) {
-        const int k = u / kQuads * kLines + l;
-        const bool ok = k0 + k < end && o.has(k0 + k);
-        const T* q = p + k * step + c;
+      for (int i = 0; i < kUnits; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[i][l][e] = ok && c + e < o.cols ? q[e] : (T)0.0f;
+        for (int l = 0; l < 4; l++) v[i][l] = *reinterpret_cast<const u32x2*>(o.p + (k0 + l) * o.stride + off[i]);
+    } else {
+      load(o, k0, k0 + kDepth<T>);
+    }
+  }
+  __device__ __forceinline__ void load(const Op& o, long k0, long end) {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++) {
+      const int left = o.cols - o.col0 - unit(i) % kWidth * kCols;
+#pragma unroll
+      for (int l = 0; l < 4; l++) {
+        const T* p = o.p + (k0 + l) * o.stride + off[i];
+        const bool ok = k0 + unit(i) / kWidth * 4 + l < end;
+        unsigned w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < kCols; e++)
+          if (ok && e < left) w[e * sizeof(T) / 4] |= bits(p[e]) << (e * sizeof(T) % 4 * 8);
+        v[i][l] = u32x2{w[0], w[1]};
       }
     }
   }
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const int u = threadIdx.x + i * THREADS, row = u % kQuads * 4, part = u / kQuads;
+      const int row = unit(i) % kWidth * kCols, part = unit(i) / kWidth;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
+      for (int e = 0; e < kCols; e++) {
+        char* to = lds + lds_at<T>(ROWS, 0, row + e, part >> 1) + (part & 1) * 8;
         if constexpr (sizeof(T) == 4) {
-          const float x[4] = {v[i][0][e], v[i][1][e], v[i][2][e], v[i][3][e]};
+          float x[4];
+#pragma unroll
+          for (int l = 0; l < 4; l++) x[l] = __uint_as_float(v[i][l][e]);
           unsigned h[3][2];
           split(x, h[0], h[1], h[2]);
 #pragma unroll
-          for (int p = 0; p < 3; p++)
-            *reinterpret_cast<u32x2*>(lds + lds_at<T>(ROWS, p, row + e, part >> 1) + (part & 1) * 8) = u32x2{h[p][0], h[p][1]};
+          for (int p = 0; p < 3; p++) *reinterpret_cast<u32x2*>(to + p * ROWS * kSlots<T> * 16) = u32x2{h[p][0], h[p][1]};
         } else {
-          bf16x8 h;
-#pragma unroll
-          for (int l = 0; l < 8; l++) h[l] = v[i][l][e];
-          *reinterpret_cast<bf16x8*>(lds + lds_at<T>(ROWS, 0, row + e, part)) = h;
+          const unsigned pick = (e & 1) ? 0x07060302u : 0x05040100u;   // the upper or the lower halves of two words
+          *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(v[i][1][e / 2], v[i][0][e / 2], pick),
+                                                __builtin_amdgcn_perm(v[i][3][e / 2], v[i][2][e / 2], pick)};
         }
       }
     }
+  }
+};
+
+// ---- staging straight into LDS: bf16 and int8 ----------------------------------------------------------------------
+// Each lane's 16 bytes go from memory to LDS without passing a register. A wave's 64 pieces lie one after the other
+// there, so the swizzle is in which chunk a lane asks for. An operand that lies across k keeps its layout, lines of k
+// with the tile's rows along them, and the fragments are transposed as they are read (ds_read_b64_tr_b16: sixteen lanes
+// bring four lines of sixteen columns, and each takes a column).
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+__device__ const i32x4 kNothing = {0, 0, 0, 0};   // what is read past the end of k
+
+template <int ROWS>
+__device__ __forceinline__ int line_swizzle(int line) {
+  return ROWS >= 128 ? (line & 3) << 2 : ((line >> 1) & 1) << 2;
+}
+
+template <typename T, typename Op, int ROWS, int THREADS>
+struct Direct {
+  static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * kSlots<T> / THREADS;
+  static_assert(ROWS * kSlots<T> % THREADS == 0, "whole units");
+  static constexpr int kLine = ROWS / kPer;   // chunks of a line (across)
+  unsigned off[kUnits];
+
+  static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
+  // k of the unit's first element (along), or its line (across), within the tile
+  static __device__ __forceinline__ int depth(int i) {
+    if constexpr (Op::kAlong) return (unit(i) % kSlots<T> ^ swizzle<T>(unit(i) / kSlots<T>)) * kPer;
+    else return unit(i) / kLine;
+  }
+  __device__ __forceinline__ void init(const Op& o) {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++) {
+      if constexpr (Op::kAlong) {
+        off[i] = o.offset(unit(i) / kSlots<T>) + depth(i);
+      } else {
+        const int c = o.col0 + (unit(i) % kLine ^ line_swizzle<ROWS>(depth(i))) * kPer;
+        off[i] = (unsigned)depth(i) * (unsigned)o.stride + (unsigned)(c < o.cols ? c : 0);
+      }
+    }
+  }
+  __device__ __forceinline__ const T* from(const Op& o, long k0, int i) const {
+    if constexpr (Op::kAlong) return o.base(__builtin_amdgcn_readfirstlane(unit(i) / kSlots<T>)) + k0 + off[i];
+    else return o.p + k0 * o.stride + off[i];
+  }
+  static __device__ __forceinline__ void piece(const void* p, char* lds, int i) {
+    char* to = lds + (i * THREADS + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * 16;
+    __builtin_amdgcn_global_load_lds((GlobalPtr)p, (LdsPtr)to, 16, 0, 0);
+  }
+  __device__ __forceinline__ void fetch(const Op& o, long k0, char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++) piece(from(o, k0, i), lds, i);
+  }
+  __device__ __forceinline__ void fetch(const Op& o, long k0, long end, char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++)
+      piece(k0 + depth(i) < end ? (const void*)from(o, k0, i) : (const void*)&kNothing, lds, i);
   }
 };
 
@@ -287,58 +347,155 @@ struct Shape {
   static constexpr int kThreads = WM * WN * 64, IM = BM / WM / 32, JN = BN / WN / 32;
 };
 
+// LDS of a block: two tiles of both operands
 template <typename T, typename S>
-constexpr int kLdsBytes = Form<T>::kPlanes * (S::BM + S::BN) * Form<T>::kRowBytes;
+struct Lds {
+  static constexpr int kA = Form<T>::kPlanes * S::BM * kSlots<T> * 16, kB = Form<T>::kPlanes * S::BN * kSlots<T> * 16;
+};
 
-// The accumulators over k in [k0, end). One LDS buffer: the next tile's global loads are in flight while this one is
-// multiplied, and the two or three blocks of a CU cover each other's barriers and stores.
+// The accumulators over k in [k0, end), with two LDS buffers and one barrier a tile. fp32: while a tile is multiplied,
+// the next one goes from registers into the other buffer (the splitting runs under the matrix instructions) and the one
+// after it is on its way from memory. bf16 and int8: while a tile is multiplied, the next one is on its way into the
+// other buffer.
 template <typename T, typename S, bool WIDE, typename OpA, typename OpB>
-__device__ __forceinline__ void multiply(const OpA& A, const OpB& B, long k0, long end, char* lds,
-                                         typename Form<T>::Acc (&acc)[S::IM][S::JN]) {
-  constexpr int P = Form<T>::kPlanes;
+struct Product {
+  static constexpr int P = Form<T>::kPlanes, D = kDepth<T>;
+  static constexpr bool kDirect = WIDE && sizeof(T) != 4;
   typedef typename Mma<T>::Op Op;
-  char* la = lds;
-  char* lb = lds + P * S::BM * Form<T>::kRowBytes;
-  Stage<T, OpA, S::BM, S::kThreads, WIDE> sa;
-  Stage<T, OpB, S::BN, S::kThreads, WIDE> sb;
-  sa.init(A);
-  sb.init(B);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int ra = wave / S::WN * S::IM * 32 + (lane & 31), rb = wave % S::WN * S::JN * 32 + (lane & 31);
-  if (k0 < end) {
-    sa.load(A, k0, end);
-    sb.load(B, k0, end);
-  }
-  for (; k0 < end; k0 += kDepth<T>) {
-    __syncthreads();
-    sa.store(la);
-    sb.store(lb);
-    __syncthreads();
-    if (k0 + kDepth<T> < end) {
-      sa.load(A, k0 + kDepth<T>, end);
-      sb.load(B, k0 + kDepth<T>, end);
+  typedef typename Form<T>::Acc Acc;
+  template <typename O, int ROWS>
+  using Mover = std::conditional_t<kDirect, Direct<T, O, ROWS, S::kThreads>, Stage<T, O, ROWS, S::kThreads, WIDE>>;
+  Mover<OpA, S::BM> sa;
+  Mover<OpB, S::BN> sb;
+
+  // the fragment of 32 rows from `row`, step s of the tile
+  template <typename O, int ROWS>
+  static __device__ __forceinline__ Op fragment(const char* lds, int p, int row, int s) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (kDirect && !O::kAlong) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* Ptr;
+      const int line = s * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2), col = row + (lane & 16) + (lane & 3) * 4;
+      const char* at = lds + ((line * (ROWS / 8)) + (col / 8 ^ line_swizzle<ROWS>(line))) * 16 + (lane & 1) * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)at);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(at + 4 * (ROWS / 8) * 16));   // the same swizzle
+      return __builtin_bit_cast(Op, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      return *reinterpret_cast<const Op*>(lds + lds_at<T>(ROWS, p, row + (lane & 31), s * 2 + (lane >> 5)));
     }
+  }
+  static __device__ __forceinline__ void step(const char* lds, int s, Acc (&acc)[S::IM][S::JN]) {
+    const int wave = threadIdx.x >> 6, ra = wave / S::WN * S::IM * 32, rb = wave % S::WN * S::JN * 32;
+    Op a[P][S::IM], b[P][S::JN];
 #pragma unroll
-    for (int s = 0; s < kSlots<T> / 2; s++) {
-      const int c = s * 2 + (lane >> 5);
-      Op a[P][S::IM], b[P][S::JN];
+    for (int p = 0; p < P; p++) {
 #pragma unroll
-      for (int p = 0; p < P; p++) {
+      for (int i = 0; i < S::IM; i++) a[p][i] = fragment<OpA, S::BM>(lds, p, ra + i * 32, s);
 #pragma unroll
-        for (int i = 0; i < S::IM; i++) a[p][i] = *reinterpret_cast<const Op*>(la + lds_at<T>(S::BM, p, ra + i * 32, c));
+      for (int j = 0; j < S::JN; j++) b[p][j] = fragment<OpB, S::BN>(lds + Lds<T, S>::kA, p, rb + j * 32, s);
+    }
+    // the planes' products, the smallest first
+    constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-        for (int j = 0; j < S::JN; j++) b[p][j] = *reinterpret_cast<const Op*>(lb + lds_at<T>(S::BN, p, rb + j * 32, c));
+    for (int q = P == 3 ? 0 : 5; q < 6; q++)
+#pragma unroll
+      for (int i = 0; i < S::IM; i++)
+#pragma unroll
+        for (int j = 0; j < S::JN; j++) acc[i][j] = Mma<T>::go(a[pa[q]][i], b[pb[q]][j], acc[i][j]);
+  }
+  static __device__ __forceinline__ void tile(const char* lds, Acc (&acc)[S::IM][S::JN]) {
+#pragma unroll
+    for (int s = 0; s < kSlots<T> / 2; s++) step(lds, s, acc);
+  }
+  // every wave's reads of this tile, and its pieces of the next one, are done
+  static __device__ __forceinline__ void turn_over() {
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void fetch(const OpA& A, const OpB& B, long k, long end, char* lds) const {
+    if (k + D <= end) {
+      sa.fetch(A, k, lds);
+      sb.fetch(B, k, lds + Lds<T, S>::kA);
+    } else {
+      sa.fetch(A, k, end, lds);
+      sb.fetch(B, k, end, lds + Lds<T, S>::kA);
+    }
+  }
+  __device__ __forceinline__ void load(const OpA& A, const OpB& B, long k, long end) {
+    if (k + D <= end) {
+      sa.load(A, k);
+      sb.load(B, k);
+    } else {
+      sa.load(A, k, end);
+      sb.load(B, k, end);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+    sa.store(lds);
+    sb.store(lds + Lds<T, S>::kA);
+  }
+
+  __device__ __forceinline__ void run(const OpA& A, const OpB& B, long k0, long end, char* lds0, char* lds1,
+                                      Acc (&acc)[S::IM][S::JN]) {
+    if (k0 >= end) return;
+    sa.init(A);
+    sb.init(B);
+    __syncthreads();   // an earlier product's reads
+    if constexpr (kDirect) {
+      fetch(A, B, k0, end, lds0);
+      turn_over();
+      for (; k0 + 3 * D <= end; k0 += 2 * D) {
+        sa.fetch(A, k0 + D, lds1);
+        sb.fetch(B, k0 + D, lds1 + Lds<T, S>::kA);
+        __builtin_amdgcn_sched_barrier(0);   // on their way first
+        tile(lds0, acc);
+        turn_over();
+        sa.fetch(A, k0 + 2 * D, lds0);
+        sb.fetch(B, k0 + 2 * D, lds0 + Lds<T, S>::kA);
+        __builtin_amdgcn_sched_barrier(0);   // on their way first
+        tile(lds1, acc);
+        turn_over();
       }
-      // the planes' products, the smallest first
-      constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-      for (int q = P == 3 ? 0 : 5; q < 6; q++)
-#pragma unroll
-        for (int i = 0; i < S::IM; i++)
-#pragma unroll
-          for (int j = 0; j < S::JN; j++) acc[i][j] = Mma<T>::go(a[pa[q]][i], b[pb[q]][j], acc[i][j]);
+      for (int odd = 0; k0 < end; k0 += D, odd ^= 1) {
+        if (k0 + D < end) fetch(A, B, k0 + D, end, odd ? lds0 : lds1);
+        tile(odd ? lds1 : lds0, acc);
+        turn_over();
+      }
+    } else {
+      load(A, B, k0, end);
+      store(lds0);
+      if (k0 + D < end) load(A, B, k0 + D, end);
+      turn_over();
+      for (; k0 + 4 * D <= end; k0 += 2 * D) {
+        store(lds1);
+        sa.load(A, k0 + 2 * D);
+        sb.load(B, k0 + 2 * D);
+        tile(lds0, acc);
+        turn_over();
+        store(lds0);
+        sa.load(A, k0 + 3 * D);
+        sb.load(B, k0 + 3 * D);
+        tile(lds1, acc);
+        turn_over();
+      }
+      for (int odd = 0; k0 < end; k0 += D, odd ^= 1) {
+        if (k0 + D < end) {
+          store(odd ? lds0 : lds1);
+          if (k0 + 2 * D < end) load(A, B, k0 + 2 * D, end);
+        }
+        tile(odd ? lds1 : lds0, acc);
+        turn_over();
+      }
     }
   }
+};
+
+template <typename T, typename S, bool WIDE, typename OpA, typename OpB>
+__device__ __forceinline__ void multiply(const OpA& A, const OpB& B, long k0, long end, char* lds0, char* lds1,
+                                         typename Form<T>::Acc (&acc)[S::IM][S::JN]) {
+  Product<T, S, WIDE, OpA, OpB> p;
+  p.run(A, B, k0, end, lds0, lds1, acc);
 }
 
 // One output again, in plain fp32
@@ -362,10 +519,9 @@ __device__ __forceinline__ int c_col(int j) {
 }
 
 // The fp32 outputs that came out infinite or NaN, again: those of rows below `rows` and of columns that are stored
-// (a column is one of them where stored(column)).
-template <typename S, typename OpA, typename OpB, typename C>
-__device__ __forceinline__ void mend(const OpA& A, const OpB& B, long k0, long end, int rows, C stored,
-                                     f32x16 (&acc)[S::IM][S::JN]) {
+// (a column is one of them where stored(column)), by value(row, column).
+template <typename S, typename C, typename V>
+__device__ __forceinline__ void mend(int rows, C stored, V value, f32x16 (&acc)[S::IM][S::JN]) {
   float z = 0;   // stays zero unless one of them is: a multiplication each
 #pragma unroll
   for (int i = 0; i < S::IM; i++)
@@ -381,7 +537,7 @@ __device__ __forceinline__ void mend(const OpA& A, const OpB& B, long k0, long e
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const int row = c_row<S>(i, r), col = c_col<S>(j);
-        if (acc[i][j][r] * 0.0f != 0 && row < rows && stored(col)) acc[i][j][r] = again(A, row, B, col, k0, end);
+        if (acc[i][j][r] * 0.0f != 0 && row < rows && stored(col)) acc[i][j][r] = value(row, col);
       }
 }
 
