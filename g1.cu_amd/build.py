@@ -52,6 +52,9 @@ SOURCES = (
     ("nn_norm.hip", []),
     ("nn_clip.hip", []),
     ("nn_gated.hip", []),
+    ("nn_gated_fp32.hip", []),
+    ("nn_gated_bf16.hip", []),
+    ("nn_gated_q8.hip", []),
 )
 
 

@@ -1,0 +1,561 @@
+// nn_gated.h -- the gated block: y = act(x Wg^T + bg) * (x Wu^T + bu), its gradients, and the same on 8-bit rows and
+// weights.
+//
+//   g = x Wg^T + bg;  u = x Wu^T + bu;  y = act(g) u
+//   dg = dy u act'(g);  du = dy act(g);  dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x;  dbg, dbu = column sums
+//
+// Forward: one product whose tile holds both projections of its outputs; activation and product in the epilogue.
+// Backward: the same product again with an epilogue that reads dy and writes d = [dg | du] (it costs 4 K operations a
+// value and saves writing and reading g and u), then dx = d [Wg; Wu], then [dWg; dWu] = d^T x with the rows split
+// over the blocks, and a join of those parts and of the column sums in a fixed order. d is held in the tensors' type.
+#pragma once
+#include <algorithm>
+#include <initializer_list>
+
+#include "nn_gemm.h"
+
+namespace g1nn {
+
+constexpr int kActs = 4;
+
+// 1 / (1 + e^-x) with the hardware's exp2 and reciprocal: off by a few units in the last place of 1 + |x|
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
+
+// act(g), and act'(g) where it is asked for. GELU in its tanh form is g sigmoid(2 z), z = sqrt(2/pi) (g + 0.044715 g^3).
+template <bool D>
+__device__ __forceinline__ float activation(int act, float g, float& d) {
+  if (act == 0) {
+    const float p = sigmoid(g);
+    if (D) d = p * __builtin_fmaf(g, 1.0f - p, 1.0f);
+    return g * p;
+  }
+  if (act == 1) {
+    // p is 0 or 1 long before 20, and beyond it a square or a cube could leave the range
+    const float c = __builtin_amdgcn_fmed3f(g, -20.0f, 20.0f), c2 = c * c;
+    const float p = sigmoid(1.5957691216057308f * c * __builtin_fmaf(0.044715f, c2, 1.0f));
+    if (D) {
+      d = p * __builtin_fmaf(c * (1.0f - p), 1.5957691216057308f * __builtin_fmaf(0.134145f, c2, 1.0f), 1.0f);
+      d = __builtin_fmaf(0.0f, g, d);   // a NaN stays one
+    }
+    return g * p;
+  }
+  if (act == 2) {
+    const float p = sigmoid(g);
+    if (D) d = p * (1.0f - p);
+    return p;
+  }
+  const float e = g > 0 ? g : expm1f(g);
+  if (D) d = g > 0 ? 1.0f : e + 1.0f;
+  return e;
+}
+
+struct GatedArgs {
+  int M, K, F;
+  const void *x, *wg, *wu, *bg, *bu, *dy;
+  long xs, wgs, wus, dys;
+  int act;
+  void* y;
+  // backward
+  int half;                 // F rounded up to 64: d is [M][2 half]
+  void* d;
+  float* sums;              // column sums of d by rows of waves, or null
+  void *dx, *dwg, *dwu, *dbg, *dbu;
+  float* parts;             // [splits][2 half][K]
+  int splits, chunk;        // rows of a split
+  float* xparts;            // [xsplits][M][K]
+  int xsplits, xchunk;      // outputs of a split of dx
+  int sum_rows;
+  // 8-bit rows and weights
+  const float *s, *sg, *su;
+};
+
+using Large = Shape<128, 128, 2, 2, false>;
+using Small = Shape<64, 64, 2, 1, true>;
+
+// The outputs of a block: y, or d and its column sums. FULL: the tile lies within the outputs.
+template <typename T, typename O, typename S, bool GRAD, bool FULL, int ACT>
+__device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, const typename Form<T>::Acc (&acc)[S::IM][S::JN]) {
+  const int lane = threadIdx.x & 63, rows = a.M - m * S::BM;
+  // addresses in 32 bits from the tile's first row, which is the same for all lanes
+  O* y = GRAD ? nullptr : (O*)a.y + (long)m * S::BM * a.F;
+  T* to = GRAD ? (T*)a.d + (long)m * S::BM * (2 * a.half) : nullptr;
+#pragma unroll
+  for (int j = 0; j < S::JN; j += 2) {
+    const int f = f0 + (c_col<S>(j) >> 6) * 32 + (lane & 31);
+    const bool in = FULL || f < a.F;
+    const int fc = in ? f : 0;
+    float bg = 0, bu = 0, sg = 0, su = 0;
+    if constexpr (sizeof(T) == 1) {
+      bg = a.bg ? ((const float*)a.bg)[fc] : 0;
+      bu = a.bu ? ((const float*)a.bu)[fc] : 0;
+      sg = a.sg[fc];
+      su = a.su[fc];
+    } else {
+      bg = a.bg ? (float)((const T*)a.bg)[fc] : 0;
+      bu = a.bu ? (float)((const T*)a.bu)[fc] : 0;
+    }
+    float sum_g = 0, sum_u = 0;
+#pragma unroll
+    for (int i = 0; i < S::IM; i++) {
+      // what each row brings, read for sixteen rows at once
+      float given[16];
+      if constexpr (GRAD || sizeof(T) == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          int row = c_row<S>(i, r);
+          if (!FULL) row = row < rows ? row : rows - 1;
+          const long at = (long)m * S::BM + row;
+          if constexpr (GRAD) given[r] = (float)((const T*)a.dy)[at * a.dys + fc];
+          else given[r] = a.s[at];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int row = c_row<S>(i, r);
+        float g, u;
+        if constexpr (sizeof(T) == 1) {
+          g = (float)acc[i][j][r] * (given[r] * sg) + bg;
+          u = (float)acc[i][j + 1][r] * (given[r] * su) + bu;
+        } else {
+          g = acc[i][j][r] + bg;
+          u = acc[i][j + 1][r] + bu;
+        }
+        float d;
+        const float v = activation<GRAD>(ACT, g, d);
+        const bool there = FULL || row < rows;
+        if constexpr (!GRAD) {
+          if (there && in) y[(unsigned)row * (unsigned)a.F + f] = (O)(v * u);
+        } else {
+          const float dg = there && in ? given[r] * u * d : 0, du = there && in ? given[r] * v : 0;
+          const unsigned at = (unsigned)row * (2 * a.half) + f;
+          if (there) {   // the columns from F to `half` are zeros
+            to[at] = (T)dg;
+            to[at + a.half] = (T)du;
+          }
+          sum_g += dg;
+          sum_u += du;
+        }
+      }
+    }
+    if constexpr (GRAD) {
+      if (a.sums) {
+        sum_g += __shfl_xor(sum_g, 32);
+        sum_u += __shfl_xor(sum_u, 32);
+        float* at = a.sums + ((long)m * S::WM + (threadIdx.x >> 6) / S::WN) * (2 * a.half) + f;
+        if (lane < 32) {
+          at[0] = sum_g;
+          at[a.half] = sum_u;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
+__global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+  const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
+  int m, n;
+  if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
+  const int f0 = n * (S::BN / 2);
+  const Along<T> A{(const T*)a.x, a.xs, m * S::BM, a.M};
+  const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, f0, a.F};
+  typename Form<T>::Acc acc[S::IM][S::JN] = {};
+  multiply<T, S, WIDE>(A, B, 0, a.K, lds0, lds1, acc);
+  if constexpr (sizeof(T) == 4)
+    mend<S>(a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; },
+            [&](int r, int c) { return again(A, r, B, c, 0, a.K); }, acc);
+  if (m * S::BM + S::BM <= a.M && f0 + S::BN / 2 <= a.F) gated_out<T, O, S, GRAD, true, ACT>(a, m, f0, acc);
+  else gated_out<T, O, S, GRAD, false, ACT>(a, m, f0, acc);
+}
+
+// dx = d [Wg; Wu], or with xsplits > 1 its parts: part s takes the outputs [s xchunk, (s + 1) xchunk) of both projections.
+template <typename T, typename S, bool WIDE>
+__global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+  const int tm = (a.M + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
+  int m, n;
+  if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
+  const Along<T> dg{(const T*)a.d, 2l * a.half, m * S::BM, a.M}, du{dg.p + a.half, dg.stride, dg.row0, dg.rows};
+  const Across<T> wg{(const T*)a.wg, a.wgs, n * S::BN, a.K}, wu{(const T*)a.wu, a.wus, n * S::BN, a.K};
+  const int f0 = blockIdx.y * a.xchunk, f1 = min(f0 + a.xchunk, a.F);
+  typename Form<T>::Acc acc[S::IM][S::JN] = {};
+  multiply<T, S, WIDE>(dg, wg, f0, f1, lds0, lds1, acc);
+  multiply<T, S, WIDE>(du, wu, f0, f1, lds0, lds1, acc);
+  const int rows = a.M - m * S::BM, cols = a.K - n * S::BN;
+  if constexpr (sizeof(T) == 4)
+    mend<S>(rows, [&](int c) { return c < cols; },
+            [&](int r, int c) { return again(dg, r, wg, c, f0, f1) + again(du, r, wu, c, f0, f1); }, acc);
+  const long at = (long)m * S::BM * a.K + n * S::BN;
+  T* to = (T*)a.dx + at;
+  float* part = a.xparts + (long)blockIdx.y * a.M * a.K + at;
+#pragma unroll
+  for (int j = 0; j < S::JN; j++)
+#pragma unroll
+    for (int i = 0; i < S::IM; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int row = c_row<S>(i, r), col = c_col<S>(j);
+        if (row >= rows || col >= cols) continue;
+        if (a.xsplits > 1) part[(unsigned)row * (unsigned)a.K + col] = acc[i][j][r];
+        else to[(unsigned)row * (unsigned)a.K + col] = (T)acc[i][j][r];
+      }
+}
+
+// parts of [dWg; dWu] = d^T x: split s takes the rows [s chunk, (s + 1) chunk). Where the
+// splits are a multiple of 8, the blocks of one run on one XCD, which then reads those rows of d and x from memory once.
+template <typename T, typename S, bool WIDE>
+__global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
+  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+  const int tm = (2 * a.half + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
+  int split, t;
+  if (a.splits % 8 == 0) {
+    split = blockIdx.x / 8 / (tm * tn) * 8 + (blockIdx.x & 7);
+    t = blockIdx.x / 8 % (tm * tn);
+  } else {
+    split = blockIdx.x / (tm * tn);
+    t = blockIdx.x % (tm * tn);
+  }
+  const int m = t / tn, n = t % tn;
+  const Across<T> A{(const T*)a.d, 2l * a.half, m * S::BM, 2 * a.half};
+  const Across<T> B{(const T*)a.x, a.xs, n * S::BN, a.K};
+  const long k0 = (long)split * a.chunk, end = k0 + a.chunk < a.M ? k0 + a.chunk : a.M;
+  typename Form<T>::Acc acc[S::IM][S::JN] = {};
+  multiply<T, S, WIDE>(A, B, k0, end, lds0, lds1, acc);
+  const int rows = 2 * a.half - m * S::BM, cols = a.K - n * S::BN;
+  if constexpr (sizeof(T) == 4)
+    mend<S>(rows, [&](int c) { return c < cols; }, [&](int r, int c) { return again(A, r, B, c, k0, end); }, acc);
+  float* to = a.parts + ((long)split * (2 * a.half) + m * S::BM) * a.K + n * S::BN;
+#pragma unroll
+  for (int j = 0; j < S::JN; j++)
+#pragma unroll
+    for (int i = 0; i < S::IM; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int row = c_row<S>(i, r), col = c_col<S>(j);
+        if (row < rows && col < cols) to[(unsigned)row * (unsigned)a.K + col] = acc[i][j][r];
+      }
+}
+
+// The parts joined, each in a fixed order: blocks [0, wide) take 1024 weights each, the next `deep` ones 1024 values of dx,
+// the others 16 biases each with 64 lanes to the rows of sums.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, int wide, int deep) {
+  int b = blockIdx.x;
+  if (b < wide + deep) {
+    const long i = (long)(b < wide ? b : b - wide) * 1024 + threadIdx.x;
+    const float* from;
+    T* to;
+    long step;
+    int n;
+    if (b < wide) {
+      const long each = (long)a.F * a.K;
+      if (i >= 2 * each) return;
+      const bool up = i >= each;
+      const long at = up ? i - each : i;
+      from = a.parts + at + (up ? (long)a.half * a.K : 0);
+      step = 2l * a.half * a.K;
+      to = (T*)(up ? a.dwu : a.dwg);
+      if (!to) return;
+      to += at;
+      n = a.splits;
+    } else {
+      step = (long)a.M * a.K;
+      if (i >= step) return;
+      from = a.xparts + i;
+      to = (T*)a.dx + i;
+      n = a.xsplits;
+    }
+    float v = 0;
+#pragma unroll 4
+    for (int s = 0; s < n; s++) v += from[s * step];
+    *to = (T)v;
+    return;
+  }
+  b -= wide + deep;
+  __shared__ float part[64][17];
+  const int c = threadIdx.x & 15, o = threadIdx.x >> 4, i = b * 16 + c;
+  const bool up = i >= a.half;
+  const int f = up ? i - a.half : i;
+  T* to = (T*)(up ? a.dbu : a.dbg);
+  float v = 0;
+  if (to && f < a.F) {
+    const float* from = a.sums + i;
+    const long step = 2l * a.half;
+#pragma unroll 8
+    for (int p = o; p < a.sum_rows; p += 64) v += from[p * step];
+  }
+  part[o][c] = v;
+  __syncthreads();
+  if (o == 0 && to && f < a.F) {
+    for (int p = 1; p < 64; p++) v += part[p][c];
+    to[f] = (T)v;
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------
+// Up to 8 rows: a wave takes an output, reads its two rows of weights once, 16 bytes a lane, and multiplies all of
+// the rows of x with them. Bound by the weights' way from memory; matrix tiles would be mostly padding.
+template <typename T>
+struct Dot {
+  static constexpr int kVec = 16 / sizeof(T);
+  typedef float Acc;
+  template <int VEC>
+  static __device__ __forceinline__ void load(const T* p, float (&o)[VEC]) { Elems<T, VEC>::load(p, o); }
+  template <int VEC>
+  static __device__ __forceinline__ void add(const float (&a)[VEC], const float (&b)[VEC], float& c) {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) c = __builtin_fmaf(a[i], b[i], c);
+  }
+  template <int VEC>
+  using Held = float[VEC];
+};
+template <>
+struct Dot<i8> {
+  static constexpr int kVec = 16;
+  typedef int Acc;
+  template <int VEC>
+  using Held = int[VEC == 1 ? 1 : VEC / 4];
+  template <int N>
+  static __device__ __forceinline__ void load(const i8* p, int (&o)[N]) {
+    if constexpr (N == 1) {
+      o[0] = *p;
+    } else {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = v[i];
+    }
+  }
+  template <int N>
+  static __device__ __forceinline__ void add(const int (&a)[N], const int (&b)[N], int& c) {
+    if constexpr (N == 1) {
+      c += a[0] * b[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) c = __builtin_amdgcn_sdot4(a[i], b[i], c, false);
+    }
+  }
+};
+
+template <typename T, typename O, int ROWS, bool WIDE, bool GRAD>
+__global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
+  typedef typename Dot<T>::Acc Acc;
+  constexpr int VEC = WIDE ? Dot<T>::kVec : 1;
+  const int lane = threadIdx.x & 63, f = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (f >= (GRAD ? a.half : a.F)) return;
+  const bool in = f < a.F;
+  const T* wg = (const T*)a.wg + (in ? f : 0) * a.wgs;
+  const T* wu = (const T*)a.wu + (in ? f : 0) * a.wus;
+  Acc g[ROWS] = {}, u[ROWS] = {};
+#pragma unroll 2
+  for (int k = lane * VEC; k < a.K; k += 64 * VEC) {
+    typename Dot<T>::template Held<VEC> p, q, x;
+    Dot<T>::load(wg + k, p);
+    Dot<T>::load(wu + k, q);
+#pragma unroll
+    for (int m = 0; m < ROWS; m++) {
+      Dot<T>::load((const T*)a.x + (m < a.M ? m : 0) * a.xs + k, x);
+      Dot<T>::add(p, x, g[m]);
+      Dot<T>::add(q, x, u[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; m++)
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      g[m] += __shfl_xor(g[m], d);
+      u[m] += __shfl_xor(u[m], d);
+    }
+  // lane m takes row m
+  Acc gm = g[0], um = u[0];
+#pragma unroll
+  for (int m = 1; m < ROWS; m++) {
+    gm = lane == m ? g[m] : gm;
+    um = lane == m ? u[m] : um;
+  }
+  float dg = 0, du = 0;
+  if (lane < a.M) {
+    float gate, up;
+    if constexpr (sizeof(T) == 1) {
+      const float s = a.s[lane];
+      gate = (float)gm * (s * a.sg[f]) + (a.bg ? ((const float*)a.bg)[f] : 0);
+      up = (float)um * (s * a.su[f]) + (a.bu ? ((const float*)a.bu)[f] : 0);
+    } else {
+      gate = gm + (in && a.bg ? (float)((const T*)a.bg)[f] : 0);
+      up = um + (in && a.bu ? (float)((const T*)a.bu)[f] : 0);
+    }
+    float d, v;
+    switch (a.act) {
+      case 0: v = activation<GRAD>(0, gate, d); break;
+      case 1: v = activation<GRAD>(1, gate, d); break;
+      case 2: v = activation<GRAD>(2, gate, d); break;
+      default: v = activation<GRAD>(3, gate, d);
+    }
+    if constexpr (!GRAD) {
+      ((O*)a.y)[(long)lane * a.F + f] = (O)(v * up);
+    } else {
+      if (in) {
+        const float dy = (float)((const T*)a.dy)[lane * a.dys + f];
+        dg = dy * up * d;
+        du = dy * v;
+      }
+      T* to = (T*)a.d + (long)lane * (2 * a.half) + f;   // zeros from F to `half`
+      to[0] = (T)dg;
+      to[a.half] = (T)du;
+    }
+  }
+  if constexpr (GRAD) {
+    if (a.sums) {
+#pragma unroll
+      for (int d = 1; d < 8; d *= 2) {
+        dg += __shfl_xor(dg, d);
+        du += __shfl_xor(du, d);
+      }
+      if (lane == 0) {
+        a.sums[f] = dg;
+        a.sums[a.half + f] = du;
+      }
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+// Tiles of 128 x 128 where they give every CU one; else of 64 x 64, four times as many.
+inline bool large(long m, long n) { return ((m + 127) / 128) * ((n + 127) / 128) >= 256; }
+
+template <typename T, typename O, typename S, bool GRAD, int ACT>
+int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
+  const dim3 grid(tile_grid((a.M + S::BM - 1) / S::BM, ((GRAD ? a.half : a.F) + S::BN / 2 - 1) / (S::BN / 2)));
+  if (wide) return launch(k_gated<T, O, S, true, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
+  return launch(k_gated<T, O, S, false, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
+}
+
+template <typename T, typename O, bool GRAD, int ACT>
+int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
+  if (large(a.M, 2l * a.F)) return run_gated<T, O, Large, GRAD, ACT>(a, wide, st);
+  return run_gated<T, O, Small, GRAD, ACT>(a, wide, st);
+}
+
+template <typename T, typename O, int ROWS, bool GRAD>
+int run_few(const GatedArgs& a, bool wide, hipStream_t st) {
+  const dim3 grid(((GRAD ? a.half : a.F) + 3) / 4);
+  if (wide) return launch(k_gated_few<T, O, ROWS, true, GRAD>, grid, dim3(256), st, a);
+  return launch(k_gated_few<T, O, ROWS, false, GRAD>, grid, dim3(256), st, a);
+}
+
+constexpr int kFew = 8;
+
+template <typename T, typename O, bool GRAD>
+int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
+  if (a.M <= kFew) {
+    if (a.M == 1) return run_few<T, O, 1, GRAD>(a, wide, st);
+    if (a.M == 2) return run_few<T, O, 2, GRAD>(a, wide, st);
+    if (a.M <= 4) return run_few<T, O, 4, GRAD>(a, wide, st);
+    return run_few<T, O, 8, GRAD>(a, wide, st);
+  }
+  switch (a.act) {
+    case 0: return run_gated<T, O, GRAD, 0>(a, wide, st);
+    case 1: return run_gated<T, O, GRAD, 1>(a, wide, st);
+    case 2: return run_gated<T, O, GRAD, 2>(a, wide, st);
+    default: return run_gated<T, O, GRAD, 3>(a, wide, st);
+  }
+}
+
+template <typename T, typename S>
+int run_dx(const GatedArgs& a, bool wide, hipStream_t st) {
+  const dim3 grid(tile_grid((a.M + S::BM - 1) / S::BM, (a.K + S::BN - 1) / S::BN), a.xsplits);
+  if (wide) return launch(k_gated_dx<T, S, true>, grid, dim3(S::kThreads), st, a);
+  return launch(k_gated_dx<T, S, false>, grid, dim3(S::kThreads), st, a);
+}
+
+template <typename T, typename S>
+int run_dw(const GatedArgs& a, bool wide, hipStream_t st) {
+  const dim3 grid((unsigned)(a.splits * ((2 * a.half + S::BM - 1) / S::BM) * (long)((a.K + S::BN - 1) / S::BN)));
+  if (wide) return launch(k_gated_dw<T, S, true>, grid, dim3(S::kThreads), st, a);
+  return launch(k_gated_dw<T, S, false>, grid, dim3(S::kThreads), st, a);
+}
+
+// How the long sums are split. [dWg; dWu] over the rows: as many parts as give two blocks to each CU, of 256 rows at
+// least, and a multiple of eight (one L2 each) from three on. dx over the outputs, only where its tiles leave CUs idle:
+// parts of 128 outputs of both projections at least.
+struct Split {
+  int half, splits, chunk, xsplits, xchunk;
+  bool large, xlarge;
+  Split(long M, int K, int F) {
+    half = (F + 63) / 64 * 64;
+    const long t128 = ((2l * half + 127) / 128) * ((K + 127) / 128), t64 = (2l * half / 64) * ((K + 63) / 64);
+    large = t128 * ((M + 255) / 256) >= 512;
+    const long tiles = large ? t128 : t64, most = (M + 255) / 256;
+    long s = (512 + tiles - 1) / tiles;
+    if (s > 2) s = (s + 7) / 8 * 8;
+    s = std::max(1l, std::min(s, most));
+    chunk = (int)std::max(64l, ((M + s - 1) / s + 63) / 64 * 64);
+    splits = (int)((M + chunk - 1) / chunk);
+    xlarge = g1nn::large(M, K);
+    const long x = xlarge ? 256 : ((M + 63) / 64) * ((K + 63) / 64);
+    s = x > 0 ? std::max(1l, std::min(256 / x, (F + 127l) / 128)) : 1;
+    xchunk = (int)(((F + s - 1) / s + 63) / 64 * 64);
+    xsplits = (F + xchunk - 1) / xchunk;
+  }
+};
+
+inline long round16(long n) { return (n + 15) / 16 * 16; }
+
+struct Workspace {
+  long d, sums, parts, xparts, bytes;
+  Workspace(int type, long M, int K, const Split& s) {
+    d = 0;
+    sums = d + round16(M * 2 * s.half * (type == 0 ? 4 : 2));
+    // rows of column sums: ceil(M / BM) WM of them, two for every 128 rows with large tiles, four with small ones
+    parts = sums + round16((M + 127) / 128 * 4 * 2 * s.half * 4);
+    xparts = parts + round16((long)s.splits * 2 * s.half * K * 4);
+    bytes = xparts + (s.xsplits > 1 ? s.xsplits * M * K * 4 : 0);
+  }
+};
+
+// Whether rows of n elements can be read in accesses of `bytes`.
+inline bool even(const void* p, long stride, long n, int size, int bytes) {
+  return aligned(p, bytes) && stride * size % bytes == 0 && n * size % bytes == 0;
+}
+
+template <typename T>
+int gated_backward(GatedArgs a, const Split& s, hipStream_t st) {
+  const int size = sizeof(T);
+  const bool xw = even(a.x, a.xs, a.K, size, 16);
+  const bool wide = xw && even(a.wg, a.wgs, a.K, size, 16) && even(a.wu, a.wus, a.K, size, 16);
+  const bool weights = a.dwg || a.dwu, biases = a.dbg || a.dbu;
+  if (!biases) a.sums = nullptr;
+  const bool big = large(a.M, 2l * a.F);
+  a.sum_rows = a.M <= kFew ? 1 : big ? (a.M + Large::BM - 1) / Large::BM * Large::WM : (a.M + Small::BM - 1) / Small::BM * Small::WM;
+  if (a.M > 0) {
+    int rc = run_gated<T, T, true>(a, wide, st);
+    if (rc) return rc;
+    if (a.dx) {
+      rc = s.xlarge ? run_dx<T, Large>(a, wide, st) : run_dx<T, Small>(a, wide, st);
+      if (rc) return rc;
+    }
+    if (weights) {
+      rc = s.large ? run_dw<T, Large>(a, xw, st) : run_dw<T, Small>(a, xw, st);
+      if (rc) return rc;
+    }
+  } else {
+    a.splits = a.sum_rows = 0;
+  }
+  const bool parted = a.M > 0 && a.dx && a.xsplits > 1;
+  if (!weights && !biases && !parted) return 0;
+  const long nw = weights ? (2l * a.F * a.K + 1023) / 1024 : 0, nb = biases ? 2 * a.half / 16 : 0,
+             nx = parted ? ((long)a.M * a.K + 1023) / 1024 : 0;
+  return launch(k_gated_join<T>, dim3((unsigned)(nw + nx + nb)), dim3(1024), st, a, (int)nw, (int)nx);
+}
+
+// One translation unit each for fp32, bf16 and 8 bits.
+extern template int run_gated<float, float, false>(const GatedArgs&, bool, hipStream_t);
+extern template int run_gated<bf16, bf16, false>(const GatedArgs&, bool, hipStream_t);
+extern template int run_gated<i8, float, false>(const GatedArgs&, bool, hipStream_t);
+extern template int run_gated<i8, bf16, false>(const GatedArgs&, bool, hipStream_t);
+extern template int gated_backward<float>(GatedArgs, const Split&, hipStream_t);
+extern template int gated_backward<bf16>(GatedArgs, const Split&, hipStream_t);
+
+}  // namespace g1nn

@@ -10,7 +10,7 @@
 // one, so six products beat one. Where a sum comes out infinite or NaN (an operand was, or was too large to round to
 // bf16: a rest of an infinity is NaN), that output is summed again in plain fp32, so it is what the formula gives.
 //
-// LDS. A tile's row has kSlots chunks; a chunk c lies in the row's slot c ^ (some bits of the row), so that the sixteen
+// LDS. A tile's row has 2, 4 or 8 chunks; a chunk c lies in the row's slot c ^ (some bits of the row), so that the sixteen
 // rows of a phase of a 16-byte read fall into different banks (64 of them: 256 bytes a cycle).
 #pragma once
 #include <type_traits>
@@ -29,37 +29,33 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-// How a type goes through the matrix cores: planes in LDS, elements per 16-byte chunk, chunks of a row of a tile.
+// How a type goes through the matrix cores: planes in LDS, elements per 16-byte chunk.
 template <typename T>
 struct Form;
 template <>
 struct Form<float> {
-  static constexpr int kPlanes = 3, kPer = 8, kSlots = 2;
+  static constexpr int kPlanes = 3, kPer = 8;
   typedef f32x16 Acc;
 };
 template <>
 struct Form<bf16> {
-  static constexpr int kPlanes = 1, kPer = 8, kSlots = 8;
+  static constexpr int kPlanes = 1, kPer = 8;
   typedef f32x16 Acc;
 };
 template <>
 struct Form<i8> {
-  static constexpr int kPlanes = 1, kPer = 16, kSlots = 4;
+  static constexpr int kPlanes = 1, kPer = 16;
   typedef i32x16 Acc;
 };
 
-template <typename T>
-constexpr int kSlots = Form<T>::kSlots;
-template <typename T>
-constexpr int kDepth = kSlots<T> * Form<T>::kPer;        // k of a tile
-
-template <typename T>
+// SLOTS: 16-byte chunks of a tile's row.
+template <int SLOTS>
 __device__ __forceinline__ int swizzle(int row) {
-  return kSlots<T> == 2 ? (row >> 3) & 1 : kSlots<T> == 4 ? (row >> 2) & 3 : (row ^ (row >> 3)) & 7;
+  return SLOTS == 2 ? (row >> 3) & 1 : SLOTS == 4 ? (row >> 2) & 3 : (row ^ (row >> 3)) & 7;
 }
-template <typename T>
+template <int SLOTS>
 __device__ __forceinline__ int lds_at(int rows, int plane, int row, int c) {
-  return ((plane * rows + row) * kSlots<T> + (c ^ swizzle<T>(row))) * 16;
+  return ((plane * rows + row) * SLOTS + (c ^ swizzle<SLOTS>(row))) * 16;
 }
 
 __device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
@@ -128,24 +124,24 @@ struct Across {
 
 // ---- staging through registers: fp32, and rows that 16-byte accesses do not fit ------------------------------------
 // WIDE: the host has checked that every chunk's elements lie within the operand and can be read in aligned accesses.
-template <typename T, typename Op, int ROWS, int THREADS, bool WIDE, bool ALONG = Op::kAlong>
+template <typename T, typename Op, int ROWS, int SLOTS, int THREADS, bool WIDE, bool ALONG = Op::kAlong>
 struct Stage;
 
-template <typename T, typename Op, int ROWS, int THREADS, bool WIDE>
-struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
-  static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * kSlots<T> / THREADS, kAcc = sizeof(T) == 4 ? 2 : 1;
-  static_assert(ROWS * kSlots<T> % THREADS == 0, "whole units");
+template <typename T, typename Op, int ROWS, int SLOTS, int THREADS, bool WIDE>
+struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, true> {
+  static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * SLOTS / THREADS, kAcc = sizeof(T) == 4 ? 2 : 1;
+  static_assert(ROWS * SLOTS % THREADS == 0, "whole units");
   unsigned off[kUnits];
   i32x4 v[kUnits][kAcc];
 
   static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
   // a wave's unit lies within 32 rows: one base
   static __device__ __forceinline__ const T* base(const Op& o, int i) {
-    return o.base(__builtin_amdgcn_readfirstlane(unit(i) / kSlots<T>));
+    return o.base(__builtin_amdgcn_readfirstlane(unit(i) / SLOTS));
   }
   __device__ __forceinline__ void init(const Op& o) {
 #pragma unroll
-    for (int i = 0; i < kUnits; i++) off[i] = o.offset(unit(i) / kSlots<T>) + unit(i) % kSlots<T> * kPer;
+    for (int i = 0; i < kUnits; i++) off[i] = o.offset(unit(i) / SLOTS) + unit(i) % SLOTS * kPer;
   }
   __device__ __forceinline__ void load(const Op& o, long k0) {
     if constexpr (WIDE) {
@@ -154,7 +150,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
 #pragma unroll
         for (int a = 0; a < kAcc; a++) v[i][a] = reinterpret_cast<const i32x4*>(base(o, i) + k0 + off[i])[a];
     } else {
-      load(o, k0, k0 + kDepth<T>);
+      load(o, k0, k0 + SLOTS * Form<T>::kPer);
     }
   }
   // zeros from `end`
@@ -162,7 +158,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       const T* p = base(o, i) + k0 + off[i];
-      const int n = (int)(end - k0) - unit(i) % kSlots<T> * kPer;
+      const int n = (int)(end - k0) - unit(i) % SLOTS * kPer;
       constexpr int kIn = 4 / sizeof(T);   // elements of a word
 #pragma unroll
       for (int w = 0; w < kPer / kIn; w++) {
@@ -177,8 +173,8 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
-      const int row = unit(i) / kSlots<T>, c = unit(i) % kSlots<T>;
-      char* to = lds + lds_at<T>(ROWS, 0, row, c);
+      const int row = unit(i) / SLOTS, c = unit(i) % SLOTS;
+      char* to = lds + lds_at<SLOTS>(ROWS, 0, row, c);
       if constexpr (sizeof(T) == 4) {
         float x[8];
 #pragma unroll
@@ -187,7 +183,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
         split(x, h[0], h[1], h[2]);
 #pragma unroll
         for (int p = 0; p < 3; p++)
-          *reinterpret_cast<u32x4*>(to + p * ROWS * kSlots<T> * 16) = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
+          *reinterpret_cast<u32x4*>(to + p * ROWS * SLOTS * 16) = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
       } else {
         *reinterpret_cast<i32x4*>(to) = v[i][0];
       }
@@ -196,10 +192,10 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, true> {
 };
 
 // Transposing: a unit is four consecutive memory rows (half a chunk) of two fp32 or four bf16 columns.
-template <typename T, typename Op, int ROWS, int THREADS, bool WIDE>
-struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
-  static constexpr int kCols = 8 / sizeof(T), kWidth = ROWS / kCols, kUnits = kWidth * (kDepth<T> / 4) / THREADS;
-  static_assert(kWidth * (kDepth<T> / 4) % THREADS == 0, "whole units");
+template <typename T, typename Op, int ROWS, int SLOTS, int THREADS, bool WIDE>
+struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, false> {
+  static constexpr int kCols = 8 / sizeof(T), kWidth = ROWS / kCols, kUnits = kWidth * (SLOTS * Form<T>::kPer / 4) / THREADS;
+  static_assert(kWidth * (SLOTS * Form<T>::kPer / 4) % THREADS == 0, "whole units");
   unsigned off[kUnits];
   u32x2 v[kUnits][4];
 
@@ -219,7 +215,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
 #pragma unroll
         for (int l = 0; l < 4; l++) v[i][l] = *reinterpret_cast<const u32x2*>(o.p + (k0 + l) * o.stride + off[i]);
     } else {
-      load(o, k0, k0 + kDepth<T>);
+      load(o, k0, k0 + SLOTS * Form<T>::kPer);
     }
   }
   __device__ __forceinline__ void load(const Op& o, long k0, long end) {
@@ -244,7 +240,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
       const int row = unit(i) % kWidth * kCols, part = unit(i) / kWidth;
 #pragma unroll
       for (int e = 0; e < kCols; e++) {
-        char* to = lds + lds_at<T>(ROWS, 0, row + e, part >> 1) + (part & 1) * 8;
+        char* to = lds + lds_at<SLOTS>(ROWS, 0, row + e, part >> 1) + (part & 1) * 8;
         if constexpr (sizeof(T) == 4) {
           float x[4];
 #pragma unroll
@@ -252,7 +248,7 @@ struct Stage<T, Op, ROWS, THREADS, WIDE, false> {
           unsigned h[3][2];
           split(x, h[0], h[1], h[2]);
 #pragma unroll
-          for (int p = 0; p < 3; p++) *reinterpret_cast<u32x2*>(to + p * ROWS * kSlots<T> * 16) = u32x2{h[p][0], h[p][1]};
+          for (int p = 0; p < 3; p++) *reinterpret_cast<u32x2*>(to + p * ROWS * SLOTS * 16) = u32x2{h[p][0], h[p][1]};
         } else {
           const unsigned pick = (e & 1) ? 0x07060302u : 0x05040100u;   // the upper or the lower halves of two words
           *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(v[i][1][e / 2], v[i][0][e / 2], pick),
@@ -277,24 +273,24 @@ __device__ __forceinline__ int line_swizzle(int line) {
   return ROWS >= 128 ? (line & 3) << 2 : ((line >> 1) & 1) << 2;
 }
 
-template <typename T, typename Op, int ROWS, int THREADS>
+template <typename T, typename Op, int ROWS, int SLOTS, int THREADS>
 struct Direct {
-  static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * kSlots<T> / THREADS;
-  static_assert(ROWS * kSlots<T> % THREADS == 0, "whole units");
+  static constexpr int kPer = Form<T>::kPer, kUnits = ROWS * SLOTS / THREADS;
+  static_assert(ROWS * SLOTS % THREADS == 0, "whole units");
   static constexpr int kLine = ROWS / kPer;   // chunks of a line (across)
   unsigned off[kUnits];
 
   static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
   // k of the unit's first element (along), or its line (across), within the tile
   static __device__ __forceinline__ int depth(int i) {
-    if constexpr (Op::kAlong) return (unit(i) % kSlots<T> ^ swizzle<T>(unit(i) / kSlots<T>)) * kPer;
+    if constexpr (Op::kAlong) return (unit(i) % SLOTS ^ swizzle<SLOTS>(unit(i) / SLOTS)) * kPer;
     else return unit(i) / kLine;
   }
   __device__ __forceinline__ void init(const Op& o) {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       if constexpr (Op::kAlong) {
-        off[i] = o.offset(unit(i) / kSlots<T>) + depth(i);
+        off[i] = o.offset(unit(i) / SLOTS) + depth(i);
       } else {
         const int c = o.col0 + (unit(i) % kLine ^ line_swizzle<ROWS>(depth(i))) * kPer;
         off[i] = (unsigned)depth(i) * (unsigned)o.stride + (unsigned)(c < o.cols ? c : 0);
@@ -302,7 +298,7 @@ struct Direct {
     }
   }
   __device__ __forceinline__ const T* from(const Op& o, long k0, int i) const {
-    if constexpr (Op::kAlong) return o.base(__builtin_amdgcn_readfirstlane(unit(i) / kSlots<T>)) + k0 + off[i];
+    if constexpr (Op::kAlong) return o.base(__builtin_amdgcn_readfirstlane(unit(i) / SLOTS)) + k0 + off[i];
     else return o.p + k0 * o.stride + off[i];
   }
   static __device__ __forceinline__ void piece(const void* p, char* lds, int i) {
@@ -340,17 +336,22 @@ struct Mma<i8> {
   }
 };
 
-// A block's tile is BM x BN, on WM x WN waves of IM x JN accumulators of 32 x 32.
-template <int BM_, int BN_, int WM_, int WN_>
+// A block's tile is BM x BN, on WM x WN waves of IM x JN accumulators of 32 x 32. Its depth in 16-byte chunks goes by type:
+// two chunks of fp32 planes, or four (DEEP); eight of bf16, four of int8.
+template <int BM_, int BN_, int WM_, int WN_, bool DEEP_>
 struct Shape {
+  static constexpr bool DEEP = DEEP_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kThreads = WM * WN * 64, IM = BM / WM / 32, JN = BN / WN / 32;
 };
 
+template <typename T, typename S>
+constexpr int slots = sizeof(T) == 4 ? (S::DEEP ? 4 : 2) : sizeof(T) == 2 ? 8 : 4;
+
 // LDS of a block: two tiles of both operands
 template <typename T, typename S>
 struct Lds {
-  static constexpr int kA = Form<T>::kPlanes * S::BM * kSlots<T> * 16, kB = Form<T>::kPlanes * S::BN * kSlots<T> * 16;
+  static constexpr int kA = Form<T>::kPlanes * S::BM * slots<T, S> * 16, kB = Form<T>::kPlanes * S::BN * slots<T, S> * 16;
 };
 
 // The accumulators over k in [k0, end), with two LDS buffers and one barrier a tile. fp32: while a tile is multiplied,
@@ -359,12 +360,13 @@ struct Lds {
 // other buffer.
 template <typename T, typename S, bool WIDE, typename OpA, typename OpB>
 struct Product {
-  static constexpr int P = Form<T>::kPlanes, D = kDepth<T>;
+  static constexpr int P = Form<T>::kPlanes, kSlots = slots<T, S>, D = kSlots * Form<T>::kPer;
   static constexpr bool kDirect = WIDE && sizeof(T) != 4;
   typedef typename Mma<T>::Op Op;
   typedef typename Form<T>::Acc Acc;
   template <typename O, int ROWS>
-  using Mover = std::conditional_t<kDirect, Direct<T, O, ROWS, S::kThreads>, Stage<T, O, ROWS, S::kThreads, WIDE>>;
+  using Mover = std::conditional_t<kDirect, Direct<T, O, ROWS, kSlots, S::kThreads>,
+                                   Stage<T, O, ROWS, kSlots, S::kThreads, WIDE>>;
   Mover<OpA, S::BM> sa;
   Mover<OpB, S::BN> sb;
 
@@ -381,7 +383,7 @@ struct Product {
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(at + 4 * (ROWS / 8) * 16));   // the same swizzle
       return __builtin_bit_cast(Op, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const Op*>(lds + lds_at<T>(ROWS, p, row + (lane & 31), s * 2 + (lane >> 5)));
+      return *reinterpret_cast<const Op*>(lds + lds_at<kSlots>(ROWS, p, row + (lane & 31), s * 2 + (lane >> 5)));
     }
   }
   static __device__ __forceinline__ void step(const char* lds, int s, Acc (&acc)[S::IM][S::JN]) {
@@ -405,7 +407,7 @@ struct Product {
   }
   static __device__ __forceinline__ void tile(const char* lds, Acc (&acc)[S::IM][S::JN]) {
 #pragma unroll
-    for (int s = 0; s < kSlots<T> / 2; s++) step(lds, s, acc);
+    for (int s = 0; s < kSlots / 2; s++) step(lds, s, acc);
   }
   // every wave's reads of this tile, and its pieces of the next one, are done
   static __device__ __forceinline__ void turn_over() {
@@ -541,14 +543,14 @@ __device__ __forceinline__ void mend(int rows, C stored, V value, f32x16 (&acc)[
       }
 }
 
-// Blocks to tiles (rows of tiles `tm`, `tn` in each): block b runs on XCD b mod 8, and a row of tiles stays on one
-// XCD, so that its part of A is read from memory by one L2 only.
+// Blocks to tiles (`tm` rows of `tn` tiles). Block b runs on XCD b mod 8; where there are enough rows of tiles for the eight
+// to share them evenly, a row stays on one XCD, so that its part of A is read from memory by one L2 only.
 __device__ __forceinline__ bool tile_of(int b, int tm, int tn, int& m, int& n) {
-  const int i = b >> 3;
-  m = i / tn * 8 + (b & 7);
+  const int i = tm >= 64 ? b >> 3 : b;
+  m = tm >= 64 ? i / tn * 8 + (b & 7) : i / tn;
   n = i % tn;
   return m < tm;
 }
-inline unsigned tile_grid(long tm, long tn) { return (unsigned)((tm + 7) / 8 * 8 * tn); }
+inline unsigned tile_grid(long tm, long tn) { return (unsigned)((tm >= 64 ? (tm + 7) / 8 * 8 : tm) * tn); }
 
 }  // namespace g1nn
