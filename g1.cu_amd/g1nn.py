@@ -12,6 +12,7 @@ type in a call; rows have contiguous elements, and a two-dimensional input may h
 current stream, outputs and workspaces come from torch's allocator, and nothing waits for the GPU. An argument that a
 kernel does not take raises ValueError, a failed launch RuntimeError; there is no fallback path.
 """
+import array
 import ctypes
 
 import torch
@@ -41,27 +42,31 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2, "elu": 3}
 _TYPE = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _call(device, fn, *args):
-    """Run an entry point on `device`'s current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream)
+_TYPE_OF = _TYPE.get
+_stream_of = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(i).cuda_stream, a twentieth of its time
+_device_now = torch._C._cuda_getDevice
+
+
+def _run(index, fn, *args):
+    """Run an entry point on the current stream of device `index`."""
+    if index == _device_now():
+        rc = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream_of(index))
     if rc == -1:
         raise ValueError("refused by libg1env.so (the reason is on stderr)")
     if rc:
         raise RuntimeError("a kernel launch failed (the reason is on stderr)")
 
 
-def _want(t, name, device, dtype, shape=None):
+def _want(t, name, index, dtype, shape=None):
     """Check a tensor's place, type and shape."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} is not a tensor")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dtype != dtype:
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    if t.dtype is not dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
@@ -71,30 +76,32 @@ def _first(x, name="x"):
     """The type code of the tensor that the others have to go with."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} is not a tensor on a GPU")
-    if x.dtype not in _TYPE:
+    code = _TYPE_OF(x.dtype)
+    if code is None:
         raise ValueError(f"{name} is {x.dtype}: float32 and bfloat16 are supported")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} has no row elements")
-    return _TYPE[x.dtype]
+    return code
 
 
-def _vector(t, name, device, dtype, n):
-    """Address of a contiguous vector [n], or None."""
+def _vector(t, name, index, dtype, shape):
+    """Address of a contiguous vector, or None."""
     if t is None:
         return None
-    _want(t, name, device, dtype, (n,))
-    if n > 1 and t.stride(0) != 1:
+    _want(t, name, index, dtype, shape)
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
 def _stride(t, name):
     """Elements from row to row of t seen as rows of its last dimension."""
-    K = t.shape[-1]
     if t.is_contiguous():
-        return K
-    if t.dim() == 2 and (K == 1 or t.stride(1) == 1):
-        return t.stride(0)
+        return t.shape[-1]
+    if t.dim() == 2:
+        rows, cols = t.stride()
+        if cols == 1 or t.shape[1] == 1:
+            return rows
     raise ValueError(f"{name}: rows must be contiguous, and evenly spaced")
 
 
@@ -107,26 +114,38 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _once():
+    """In a backward pass: gradients are enabled there only where a graph of it is asked for."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the gradients of g1nn's operators cannot be differentiated again (create_graph)")
+
+
 # ------------------------------------------------------------------------------------ norm
 def _norm_args(x, weight, residual):
     code = _first(x)
-    K = x.shape[-1]
-    w = _vector(weight, "weight", x.device, x.dtype, K)
+    index, dtype, shape = x.get_device(), x.dtype, x.shape
+    K = shape[-1]
+    w = _vector(weight, "weight", index, dtype, (K,))
     if w is None:
         raise ValueError("weight is not a tensor")
     xs, r, rs = _stride(x, "x"), None, 0
     if residual is not None:
-        _want(residual, "residual", x.device, x.dtype, x.shape)
+        _want(residual, "residual", index, dtype, shape)
         r, rs = residual.data_ptr(), _stride(residual, "residual")
-    return code, x.numel() // K, K, x.data_ptr(), xs, r, rs, w
+    return index, (code, x.numel() // K, K, x.data_ptr(), xs, r, rs, w)
+
+
+def _like(x):
+    """A new contiguous tensor of x's shape and type."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _norm_forward(x, weight, residual, eps, keep):
-    args = _norm_args(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    rstd = torch.empty(args[1], dtype=torch.float32, device=x.device) if keep else None
-    _call(x.device, lib.g1_nn_rms_norm, *args, eps, y.data_ptr(), _ptr(h), _ptr(rstd))
+    index, args = _norm_args(x, weight, residual)
+    y = _like(x)
+    h = _like(x) if residual is not None else None
+    rstd = x.new_empty(args[1], dtype=torch.float32) if keep else None
+    _run(index, lib.g1_nn_rms_norm, *args, eps, y.data_ptr(), _ptr(h), _ptr(rstd))
     return y, h, rstd
 
 
@@ -139,25 +158,25 @@ class _RmsNorm(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
+        _once()
         h, rstd, weight = ctx.saved_tensors
         need_x, need_w, need_r, _ = ctx.needs_input_grad
         if dy is None:
             return dh if need_x else None, None, dh if need_r else None, None
         K = h.shape[-1]
         M = h.numel() // K
+        code = _TYPE[h.dtype]
         dy = _even(dy)
         dh = None if dh is None else _even(dh)
-        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dx = _like(h)
         dw = ws = None
-        code = _TYPE[h.dtype]
         if need_w:
             dw = torch.empty_like(weight)
-            ws = torch.empty(lib.g1_nn_rms_norm_backward_workspace(code, M, K), dtype=torch.uint8, device=h.device)
-        _call(h.device, lib.g1_nn_rms_norm_backward, code, M, K, dy.data_ptr(), _stride(dy, "dy"), _ptr(dh),
-              0 if dh is None else _stride(dh, "dh"), h.data_ptr(), _stride(h, "h"), rstd.data_ptr(),
-              weight.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(ws))
+            ws = h.new_empty(lib.g1_nn_rms_norm_backward_workspace(code, M, K), dtype=torch.uint8)
+        _run(h.get_device(), lib.g1_nn_rms_norm_backward, code, M, K, dy.data_ptr(), _stride(dy, "dy"), _ptr(dh),
+             0 if dh is None else _stride(dh, "dh"), h.data_ptr(), _stride(h, "h"), rstd.data_ptr(),
+             weight.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(ws))
         return dx if need_x else None, dw, dx if need_r else None, None
 
 
@@ -172,43 +191,44 @@ def rms_norm(x, weight, eps=1e-6, residual=None):
     return y if residual is None else (y, h)
 
 
-@torch.no_grad()
 def rms_norm_q8(x, weight, eps=1e-6, residual=None):
     """rms_norm with its rows in 8 bits: (q int8, scale float32 per row), and h with a residual; q * scale stands for
     the normed row, with its largest value at 127. A row of zeros has scale 0; a row with an infinity or a NaN has q = 0
     and a scale of NaN. No gradients."""
-    args = _norm_args(x, weight, residual)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    _call(x.device, lib.g1_nn_rms_norm_q8, *args, eps, q.data_ptr(), scale.data_ptr(), _ptr(h))
+    index, args = _norm_args(x, weight, residual)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    h = _like(x) if residual is not None else None
+    _run(index, lib.g1_nn_rms_norm_q8, *args, eps, q.data_ptr(), scale.data_ptr(), _ptr(h))
     return (q, scale) if h is None else (q, scale, h)
 
 
 # ------------------------------------------------------------------------------------ gated block
 def _act(name):
-    if name not in ACTIVATIONS:
+    code = ACTIVATIONS.get(name)
+    if code is None:
         raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}")
-    return ACTIVATIONS[name]
+    return code
 
 
 def _gated_args(x, w_gate, w_up, b_gate, b_up, activation):
-    code, K = _first(x), x.shape[-1]
-    dev, dt = x.device, x.dtype
-    _want(w_gate, "w_gate", dev, dt)
-    if w_gate.dim() != 2 or w_gate.shape[0] < 1 or w_gate.shape[1] != K:
-        raise ValueError(f"w_gate has shape {tuple(w_gate.shape)}, not (F, {K})")
-    _want(w_up, "w_up", dev, dt, w_gate.shape)
-    F = w_gate.shape[0]
-    return (code, x.numel() // K, K, F, x.data_ptr(), _stride(x, "x"), w_gate.data_ptr(), _stride(w_gate, "w_gate"),
-            w_up.data_ptr(), _stride(w_up, "w_up"), _vector(b_gate, "b_gate", dev, dt, F),
-            _vector(b_up, "b_up", dev, dt, F), _act(activation))
+    code = _first(x)
+    index, dt, K = x.get_device(), x.dtype, x.shape[-1]
+    _want(w_gate, "w_gate", index, dt)
+    shape = w_gate.shape
+    if len(shape) != 2 or shape[0] < 1 or shape[1] != K:
+        raise ValueError(f"w_gate has shape {tuple(shape)}, not (F, {K})")
+    _want(w_up, "w_up", index, dt, shape)
+    F = shape[0]
+    return index, (code, x.numel() // K, K, F, x.data_ptr(), _stride(x, "x"), w_gate.data_ptr(),
+                   _stride(w_gate, "w_gate"), w_up.data_ptr(), _stride(w_up, "w_up"),
+                   _vector(b_gate, "b_gate", index, dt, (F,)), _vector(b_up, "b_up", index, dt, (F,)), _act(activation))
 
 
 def _gated_forward(x, w_gate, w_up, b_gate, b_up, activation):
-    args = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
-    y = torch.empty(x.shape[:-1] + (args[3],), dtype=x.dtype, device=x.device)
-    _call(x.device, lib.g1_nn_gated, *args, y.data_ptr())
+    index, args = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
+    y = x.new_empty(x.shape[:-1] + (args[3],))
+    _run(index, lib.g1_nn_gated, *args, y.data_ptr())
     return y
 
 
@@ -220,17 +240,15 @@ class _Gated(torch.autograd.Function):
         return _gated_forward(x, w_gate, w_up, b_gate, b_up, activation)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
-        args = _gated_args(x, w_gate, w_up, b_gate, b_up, ctx.activation)
-        code, M, K, F = args[:4]
+        _once()
+        tensors = ctx.saved_tensors
+        index, args = _gated_args(*tensors, ctx.activation)
         dy = _even(dy)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-                 for t, need in zip((x, w_gate, w_up, b_gate, b_up), ctx.needs_input_grad)]
-        ws = torch.empty(lib.g1_nn_gated_backward_workspace(code, M, K, F), dtype=torch.uint8, device=x.device)
-        _call(x.device, lib.g1_nn_gated_backward, *args, dy.data_ptr(), _stride(dy, "dy"), *[_ptr(g) for g in grads],
-              ws.data_ptr())
+        grads = [_like(t) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
+        ws = dy.new_empty(lib.g1_nn_gated_backward_workspace(*args[:4]), dtype=torch.uint8)
+        _run(index, lib.g1_nn_gated_backward, *args, dy.data_ptr(), _stride(dy, "dy"), *[_ptr(g) for g in grads],
+             ws.data_ptr())
         return (*grads, None)
 
 
@@ -238,7 +256,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """activation(x w_gate^T + b_gate) * (x w_up^T + b_up) for rows x [..., K] and weights [F, K]. Both projections,
     the activation ("silu", "gelu" in its tanh form, "sigmoid" or "elu") and the product are one kernel. Differentiable
     in all tensors; the gradients compute the projections again, so no [.., F] values are kept for them."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, b_gate, b_up)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
+                                    (b_gate is not None and b_gate.requires_grad) or
+                                    (b_up is not None and b_up.requires_grad)):
         return _Gated.apply(x, w_gate, w_up, b_gate, b_up, activation)
     return _gated_forward(x, w_gate, w_up, b_gate, b_up, activation)
 
@@ -252,69 +272,78 @@ def quantize_rows(w):
     return torch.round(w * inv[:, None]).to(torch.int8), a / 127.0
 
 
-@torch.no_grad()
 def gated_linear_q8(q, scale, w_gate_q, s_gate, w_up_q, s_up, b_gate=None, b_up=None, activation="silu",
                     dtype=torch.float32):
     """The gated block on 8-bit rows q [..., K] with a scale each (rms_norm_q8) and 8-bit weights [F, K] with a scale
     per output (quantize_rows); float32 biases; y [..., F] in dtype. The products are summed as whole numbers. No
     gradients."""
-    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.int8 or q.dim() < 1 or q.shape[-1] < 1:
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype is not torch.int8 or q.dim() < 1 or q.shape[-1] < 1:
         raise ValueError("q is not an int8 tensor of rows on a GPU")
-    if dtype not in _TYPE:
+    code = _TYPE_OF(dtype)
+    if code is None:
         raise ValueError(f"{dtype}: float32 and bfloat16 are supported")
-    dev, K, f32 = q.device, q.shape[-1], torch.float32
-    _want(scale, "scale", dev, f32, q.shape[:-1])
-    _want(w_gate_q, "w_gate_q", dev, torch.int8)
-    if w_gate_q.dim() != 2 or w_gate_q.shape[0] < 1 or w_gate_q.shape[1] != K:
-        raise ValueError(f"w_gate_q has shape {tuple(w_gate_q.shape)}, not (F, {K})")
-    _want(w_up_q, "w_up_q", dev, torch.int8, w_gate_q.shape)
-    if not (scale.is_contiguous() and w_gate_q.is_contiguous() and w_up_q.is_contiguous()):
-        raise ValueError("the scales and 8-bit weights must be contiguous")
-    F = w_gate_q.shape[0]
-    _want(s_gate, "s_gate", dev, f32)
-    _want(s_up, "s_up", dev, f32)
-    y = torch.empty(q.shape[:-1] + (F,), dtype=dtype, device=dev)
-    _call(dev, lib.g1_nn_gated_q8, _TYPE[dtype], q.numel() // K, K, F, q.data_ptr(), _stride(q, "q"), scale.data_ptr(),
-          w_gate_q.data_ptr(), _vector(s_gate, "s_gate", dev, f32, F), w_up_q.data_ptr(),
-          _vector(s_up, "s_up", dev, f32, F), _vector(b_gate, "b_gate", dev, f32, F),
-          _vector(b_up, "b_up", dev, f32, F), _act(activation), y.data_ptr())
+    index, rows, f32 = q.get_device(), q.shape, torch.float32
+    K = rows[-1]
+    _want(w_gate_q, "w_gate_q", index, torch.int8)
+    shape = w_gate_q.shape
+    if len(shape) != 2 or shape[0] < 1 or shape[1] != K:
+        raise ValueError(f"w_gate_q has shape {tuple(shape)}, not (F, {K})")
+    F = shape[0]
+    for t, name in ((scale, "scale"), (s_gate, "s_gate"), (s_up, "s_up")):
+        if t is None:
+            raise ValueError(f"{name} is not a tensor")
+    args = (code, q.numel() // K, K, F, q.data_ptr(), _stride(q, "q"), _vector(scale, "scale", index, f32, rows[:-1]),
+            _vector(w_gate_q, "w_gate_q", index, torch.int8, shape), _vector(s_gate, "s_gate", index, f32, (F,)),
+            _vector(w_up_q, "w_up_q", index, torch.int8, shape), _vector(s_up, "s_up", index, f32, (F,)),
+            _vector(b_gate, "b_gate", index, f32, (F,)), _vector(b_up, "b_up", index, f32, (F,)), _act(activation))
+    if None in args[6:11]:
+        raise ValueError("w_up_q is not a tensor")
+    y = q.new_empty(rows[:-1] + (F,), dtype=dtype)
+    _run(index, lib.g1_nn_gated_q8, *args, y.data_ptr())
     return y
 
 
 # ------------------------------------------------------------------------------------ clipping
-@torch.no_grad()
+def _table(kind, values):
+    """A C array of whole numbers, which lives as long as what is returned: (array, address)."""
+    t = array.array(kind, values)
+    return t, t.buffer_info()[0]
+
+
+def _tensors(ts, what, index):
+    codes = [_TYPE_OF(t.dtype) for t in ts]
+    for t, code in zip(ts, codes):
+        if t.get_device() != index or code is None or not t.is_contiguous():
+            raise ValueError(f"{what} on {t.device}, {t.dtype}{'' if t.is_contiguous() else ', not contiguous'}: contiguous "
+                             f"float32 and bfloat16 tensors on one GPU are supported")
+    return _table("q", [t.data_ptr() for t in ts]), _table("i", codes)
+
+
 def clip_grad_norm(grads, max_norm, out=None):
     """The Euclidean norm of all gradients together (a float32 tensor without dimensions, on the GPU), and the
     gradients times min(1, max_norm / (norm + 1e-6)): in place, or into the tensors `out` of the same shapes (float32
     or bfloat16, so 16-bit gradients can be clipped into 32-bit ones). The tensors are contiguous. The squares are summed
     in 64 bits in an order that does not change. A norm that is infinite or NaN makes the factor 0 or NaN."""
     grads = list(grads)
-    outs = grads if out is None else list(out)
-    if len(outs) != len(grads):
-        raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
     if not grads:
         raise ValueError("no gradients")
-    dev = grads[0].device
-    for name, ts in (("a gradient", grads),) + ((("an output", outs),) if out is not None else ()):
-        for t in ts:
-            if t.device != dev or not t.is_cuda:
-                raise ValueError(f"{name} is on {t.device}, not on one GPU")
-            if t.dtype not in _TYPE:
-                raise ValueError(f"{name} is {t.dtype}: float32 and bfloat16 are supported")
-            if not t.is_contiguous():
-                raise ValueError(f"{name} is not contiguous")
-    if out is not None and any(g.shape != o.shape for g, o in zip(grads, outs)):
-        raise ValueError("an output has another shape than its gradient")
+    index = grads[0].get_device()
+    if index < 0:
+        raise ValueError("the gradients are not on a GPU")
+    (pin, pin_at), (tin, tin_at) = _tensors(grads, "a gradient", index)
+    pout_at, tout_at = pin_at, tin_at
+    if out is not None:
+        out = list(out)
+        if [t.shape for t in out] != [t.shape for t in grads]:
+            raise ValueError("the outputs have other shapes than the gradients")
+        (pout, pout_at), (tout, tout_at) = _tensors(out, "an output", index)
     n = len(grads)
-    ptrs, codes = (_vp * n), (_i * n)
-    pin, tin = ptrs(*[t.data_ptr() for t in grads]), codes(*[_TYPE[t.dtype] for t in grads])
-    pout, tout = (pin, tin) if out is None else (ptrs(*[t.data_ptr() for t in outs]),
-                                                 codes(*[_TYPE[t.dtype] for t in outs]))
-    sizes = (_l * n)(*[t.numel() for t in grads])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(lib.g1_nn_clip_workspace(n), dtype=torch.uint8, device=dev)
-    _call(dev, lib.g1_nn_clip, n, pin, tin, pout, tout, sizes, max_norm, norm.data_ptr(), ws.data_ptr())
-    return norm
+    sizes, sizes_at = _table("q", [t.numel() for t in grads])
+    # the norm, and behind it the workspace
+    both = grads[0].new_empty(4 + lib.g1_nn_clip_workspace(n) // 4, dtype=torch.float32)
+    _run(index, lib.g1_nn_clip, n, pin_at, tin_at, pout_at, tout_at, sizes_at, max_norm, both.data_ptr(),
+         both.data_ptr() + 16)
+    return both[0]
 
 
 def clip_grad_norm_(parameters, max_norm):
