@@ -3,7 +3,8 @@
 //
 // Two launches per table of tensors: the blocks' sums of squares, in 64 bits (a square of any finite 32-bit value
 // fits, so the norm overflows only where it is itself too large), and the scaling, whose blocks each join those sums in
-// the same fixed order. Bound by memory: the tensors are read twice and written once.
+// the same fixed order. Bound by memory: the tensors are read twice and written once; the second reading goes backwards,
+// so that it begins with what the first one left in the caches.
 #include <algorithm>
 
 #include "../../include/g1nn.h"
@@ -13,11 +14,11 @@ namespace g1nn {
 
 constexpr int kTable = 64;          // tensors of one launch: their table travels as a kernel argument
 constexpr int kClipThreads = 256;
-constexpr int kChunk = 16384;       // elements of a block's turn
+constexpr int kLeast = 2048, kMost = 16384;   // elements of a block's turn
 constexpr int kSums = 1024;         // sums of one launch: its largest grid
 
 struct ClipTable {
-  int n, chunks;
+  int n, chunks, chunk;             // chunk: elements of a block's turn
   const void* in[kTable];
   void* out[kTable];
   long size[kTable];
@@ -49,19 +50,20 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
 template <typename T>
 __device__ __forceinline__ double squares(const T* p, long n) {
   constexpr int V = 16 / sizeof(T);
-  double s = 0;
+  double s[2] = {0, 0};
   long i = 0;
   if (((uintptr_t)p & 15) == 0) {
+#pragma unroll 4
     for (i = (long)threadIdx.x * V; i + V <= n; i += kClipThreads * V) {
       float v[V];
       Elems<T, V>::load(p + i, v);
 #pragma unroll
-      for (int j = 0; j < V; j++) s += (double)v[j] * (double)v[j];
+      for (int j = 0; j < V; j++) s[j & 1] = __builtin_fma((double)v[j], (double)v[j], s[j & 1]);
     }
     i = n / V * V;
   }
-  for (i += threadIdx.x; i < n; i += kClipThreads) s += (double)(float)p[i] * (double)(float)p[i];
-  return s;
+  for (i += threadIdx.x; i < n; i += kClipThreads) s[0] = __builtin_fma((double)(float)p[i], (double)(float)p[i], s[0]);
+  return s[0] + s[1];
 }
 
 __global__ __launch_bounds__(kClipThreads) void k_clip_sums(ClipTable t, double* sums) {
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(kClipThreads) void k_clip_sums(ClipTable t, double*
   double s = 0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const int i = tensor_of(t, c);
-    const long at = (long)(c - t.first[i]) * kChunk, left = t.size[i] - at, n = left < kChunk ? left : kChunk;
+    const long at = (long)(c - t.first[i]) * t.chunk, left = t.size[i] - at, n = left < t.chunk ? left : t.chunk;
     s += t.in_type[i] == 0 ? squares((const float*)t.in[i] + at, n) : squares((const bf16*)t.in[i] + at, n);
   }
   s = block_sum(s, part);
@@ -81,6 +83,7 @@ __device__ __forceinline__ void scale(const I* in, O* out, long n, float f) {
   constexpr int V = 16 / (sizeof(I) < sizeof(O) ? sizeof(O) : sizeof(I));
   long i = 0;
   if ((((uintptr_t)in & (V * sizeof(I) - 1)) | ((uintptr_t)out & (V * sizeof(O) - 1))) == 0) {
+#pragma unroll 4
     for (i = (long)threadIdx.x * V; i + V <= n; i += kClipThreads * V) {
       float v[V];
       Elems<I, V>::load(in + i, v);
@@ -102,9 +105,9 @@ __global__ __launch_bounds__(kClipThreads) void k_clip_scale(ClipTable t, const 
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
   float f = max_norm / (total + 1e-6f);
   f = f > 1.0f ? 1.0f : f;   // a NaN stays one
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
     const int i = tensor_of(t, c);
-    const long at = (long)(c - t.first[i]) * kChunk, left = t.size[i] - at, n = left < kChunk ? left : kChunk;
+    const long at = (long)(c - t.first[i]) * t.chunk, left = t.size[i] - at, n = left < t.chunk ? left : t.chunk;
     const void* in = t.in[i];
     void* out = t.out[i];
     const int it = t.in_type[i], ot = t.out_type[i];
@@ -142,10 +145,15 @@ extern "C" int g1_nn_clip(int n, const void* const* in, const int* in_type, void
   }
   double* sums = (double*)ws;
   int nsums = 0;
+  // a block's turn: short enough to give every CU some blocks, long enough to pay for finding its tensor
+  long total = 0;
+  for (int i = 0; i < n; i++) total += size[i];
+  const int chunk = (int)std::min<long>(kMost, std::max<long>(kLeast, total / kSums / kLeast * kLeast));
   for (int pass = 0; pass < 2; pass++) {
     for (int from = 0; from < n || from == 0; from += kTable) {
       ClipTable t;
       t.n = std::min(kTable, n - from);
+      t.chunk = chunk;
       long chunks = 0;
       for (int i = 0; i < t.n; i++) {
         t.in[i] = in[from + i];
@@ -154,7 +162,7 @@ extern "C" int g1_nn_clip(int n, const void* const* in, const int* in_type, void
         t.in_type[i] = (unsigned char)in_type[from + i];
         t.out_type[i] = (unsigned char)out_type[from + i];
         t.first[i] = (int)chunks;
-        chunks += (size[from + i] + kChunk - 1) / kChunk;
+        chunks += (size[from + i] + chunk - 1) / chunk;
         if (chunks > 0x7fffffff) return refuse("the tensors are too large") ? -1 : 0;
       }
       t.first[t.n] = t.chunks = (int)chunks;

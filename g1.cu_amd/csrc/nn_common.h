@@ -16,6 +16,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T, int VEC>
 struct Elems {
   typedef T V __attribute__((ext_vector_type(VEC)));
+  static __device__ __forceinline__ T part(V v, int i) { return v[i]; }
   static __device__ __forceinline__ void load(const T* p, float (&o)[VEC]) {
     const V v = *reinterpret_cast<const V*>(p);
 #pragma unroll
@@ -30,6 +31,8 @@ struct Elems {
 };
 template <typename T>
 struct Elems<T, 1> {
+  typedef T V;
+  static __device__ __forceinline__ T part(V v, int) { return v; }
   static __device__ __forceinline__ void load(const T* p, float (&o)[1]) { o[0] = (float)*p; }
   static __device__ __forceinline__ void store(T* p, const float (&o)[1]) { *p = (T)o[0]; }
 };

@@ -150,41 +150,55 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
 #pragma unroll
     for (int j = 0; j < VEC; j++) dw[i][j] = 0;
   }
+  // rows that leave registers for it: the next one is on its way while this one is summed, as it lies in memory
+  constexpr bool kAhead = NV * VEC <= 16;
+  typedef typename Elems<T, VEC>::V V;
+  V dyv[NV], hv[NV], dhv[NV];
+  float s = 0;
+  const long step = (long)gridDim.x * kRows;
+  auto fetch = [&](long row) {
+    s = a.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int k = (i * TPR + lane) * VEC;
+      if (k < a.K) {
+        dyv[i] = *reinterpret_cast<const V*>((const T*)a.dy + row * a.dys + k);
+        hv[i] = *reinterpret_cast<const V*>((const T*)a.h + row * a.hs + k);
+        if (a.dh) dhv[i] = *reinterpret_cast<const V*>((const T*)a.dh + row * a.dhs + k);
+      }
+    }
+  };
   int turn = 0;
-  for (long row = (long)blockIdx.x * kRows + threadIdx.x / TPR; row < a.M; row += (long)gridDim.x * kRows, turn++) {
-    const T* dy = (const T*)a.dy + row * a.dys;
-    const T* hp = (const T*)a.h + row * a.hs;
-    const float s = a.rstd[row];
-    float g[NV][VEC], h[NV][VEC];
+  long row = (long)blockIdx.x * kRows + threadIdx.x / TPR;
+  if (kAhead && row < a.M) fetch(row);
+  for (; row < a.M; row += step, turn++) {
+    if (!kAhead) fetch(row);
+    float g[NV][VEC], h[NV][VEC], e[NV][VEC];
+    const float now = s;
     float c = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int k = (i * TPR + lane) * VEC;
       if (k < a.K) {
-        Elems<T, VEC>::load(dy + k, g[i]);
-        Elems<T, VEC>::load(hp + k, h[i]);
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
-          h[i][j] *= s;
-          dw[i][j] = __builtin_fmaf(g[i][j], h[i][j], dw[i][j]);
-          g[i][j] *= w[i][j];
+          const float dy = (float)Elems<T, VEC>::part(dyv[i], j);
+          h[i][j] = (float)Elems<T, VEC>::part(hv[i], j) * now;
+          e[i][j] = a.dh ? (float)Elems<T, VEC>::part(dhv[i], j) : 0.0f;
+          dw[i][j] = __builtin_fmaf(dy, h[i][j], dw[i][j]);
+          g[i][j] = dy * w[i][j];
           c = __builtin_fmaf(g[i][j], h[i][j], c);
         }
       }
     }
+    if (kAhead && row + step < a.M) fetch(row + step);
     c = row_sum<TPR>(c, part, turn) / (float)a.K;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int k = (i * TPR + lane) * VEC;
       if (k < a.K) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) g[i][j] = s * __builtin_fmaf(-h[i][j], c, g[i][j]);
-        if (a.dh) {
-          float e[VEC];
-          Elems<T, VEC>::load((const T*)a.dh + row * a.dhs + k, e);
-#pragma unroll
-          for (int j = 0; j < VEC; j++) g[i][j] += e[j];
-        }
+        for (int j = 0; j < VEC; j++) g[i][j] = now * __builtin_fmaf(-h[i][j], c, g[i][j]) + e[i][j];
         Elems<T, VEC>::store((T*)a.dx + row * a.K + k, g[i]);
       }
     }
@@ -213,18 +227,21 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
   }
 }
 
-// dw [K] from the blocks' P rows of sums: 32 columns to a block, its eight groups of lanes each taking every eighth row
+// dw [K] from the blocks' P rows of sums: 16 columns to a block, 64 groups of lanes to the rows, so that a few turns of
+// eight loads in flight pass over them; joined in a fixed order
 template <typename T>
-__global__ __launch_bounds__(256) void k_column_join(const float* part, int P, int K, T* out) {
-  __shared__ float s[8][32];
-  const int c = threadIdx.x & 31, o = threadIdx.x >> 5, k = blockIdx.x * 32 + c;
+__global__ __launch_bounds__(1024) void k_column_join(const float* part, int P, int K, T* out) {
+  __shared__ float s[64][17];
+  const int c = threadIdx.x & 15, o = threadIdx.x >> 4, k = blockIdx.x * 16 + c;
   float v = 0;
-  if (k < K)
-    for (int p = o; p < P; p += 8) v += part[(long)p * K + k];
+  if (k < K) {
+#pragma unroll 8
+    for (int p = o; p < P; p += 64) v += part[(long)p * K + k];
+  }
   s[o][c] = v;
   __syncthreads();
   if (o == 0 && k < K) {
-    for (int i = 1; i < 8; i++) v += s[i][c];
+    for (int i = 1; i < 64; i++) v += s[i][c];
     out[k] = (T)v;
   }
 }
@@ -237,7 +254,8 @@ int by_row(int K, F f) {
   if (n <= 16) return f.template go<T, VEC, 16, 1>();
   if (n <= 64) return f.template go<T, VEC, 64, 1>();
   if (n <= 128) return f.template go<T, VEC, 64, 2>();
-  if (n <= 256) return f.template go<T, VEC, 64, 4>();
+  if (n <= 256) return f.template go<T, VEC, 256, 1>();
+  if (n <= 512) return f.template go<T, VEC, 256, 2>();
   if (n <= 1024) return f.template go<T, VEC, 256, 4>();
   if (n <= 2048) return f.template go<T, VEC, 256, 8>();
   if (n <= 8192) return f.template go<T, VEC, 1024, 8>();
@@ -351,7 +369,7 @@ extern "C" int g1_nn_rms_norm_backward(int type, long M, int K, const void* dy, 
     if (rc) return rc;
   }
   if (!dw) return 0;
-  const dim3 g((K + 31) / 32);
-  if (type == 0) return launch(k_column_join<float>, g, dim3(256), st, (const float*)ws, (int)grid, K, (float*)dw);
-  return launch(k_column_join<bf16>, g, dim3(256), st, (const float*)ws, (int)grid, K, (bf16*)dw);
+  const dim3 g((K + 15) / 16);
+  if (type == 0) return launch(k_column_join<float>, g, dim3(1024), st, (const float*)ws, (int)grid, K, (float*)dw);
+  return launch(k_column_join<bf16>, g, dim3(1024), st, (const float*)ws, (int)grid, K, (bf16*)dw);
 }
