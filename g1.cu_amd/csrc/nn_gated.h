@@ -71,8 +71,28 @@ struct GatedArgs {
   const float *s, *sg, *su;
 };
 
-using Large = Shape<128, 128, 2, 2, false>;
-using Small = Shape<64, 64, 2, 1, true>;
+// Tiles of a block by type, four chunks deep; in fp32 two chunks of three planes, and four where a block is small and waits
+// more.
+template <typename T>
+struct Tiles {
+  using Huge = Shape<256, 128, 2, 2, 4>;
+  using Large = Shape<128, 128, 2, 2, 4>;
+  using Small = Shape<64, 64, 2, 1, 4>;
+};
+template <>
+struct Tiles<float> {
+  using Huge = Shape<128, 128, 2, 2, 2>;
+  using Large = Huge;
+  using Small = Shape<64, 64, 2, 1, 4>;
+};
+
+// Which of them a product of m x n takes: the large ones where they give every CU a block, the huge ones (which read
+// less from the L2s: 96 instead of 128 rows for as many products) where they give every CU four.
+enum Size { kSmall, kLarge, kHuge };
+inline Size size_of(long m, long n) {
+  if (((m + 255) / 256) * ((n + 127) / 128) >= 1024) return kHuge;
+  return ((m + 127) / 128) * ((n + 127) / 128) >= 256 ? kLarge : kSmall;
+}
 
 // The outputs of a block: y, or d and its column sums. FULL: the tile lies within the outputs.
 template <typename T, typename O, typename S, bool GRAD, bool FULL, int ACT>
@@ -154,8 +174,8 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
 }
 
 template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
-__global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
-  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+__global__ __launch_bounds__(S::kThreads, S::kThreads == 128 ? 1 : sizeof(T) == 4 ? 3 : 2) void k_gated(GatedArgs a) {
+  G1NN_LDS(T, S, WIDE);
   const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
   int m, n;
   if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
@@ -163,7 +183,7 @@ __global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
   const Along<T> A{(const T*)a.x, a.xs, m * S::BM, a.M};
   const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, f0, a.F};
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, 0, a.K, lds0, lds1, acc);
+  multiply<T, S, WIDE>(A, B, 0, a.K, lds, acc);
   if constexpr (sizeof(T) == 4)
     mend<S>(a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; },
             [&](int r, int c) { return again(A, r, B, c, 0, a.K); }, acc);
@@ -173,8 +193,8 @@ __global__ __launch_bounds__(S::kThreads) void k_gated(GatedArgs a) {
 
 // dx = d [Wg; Wu], or with xsplits > 1 its parts: part s takes the outputs [s xchunk, (s + 1) xchunk) of both projections.
 template <typename T, typename S, bool WIDE>
-__global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
-  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+__global__ __launch_bounds__(S::kThreads, S::BM == 256 ? 2 : 1) void k_gated_dx(GatedArgs a) {
+  G1NN_LDS(T, S, WIDE);
   const int tm = (a.M + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
   int m, n;
   if (!tile_of(blockIdx.x, tm, tn, m, n)) return;
@@ -182,8 +202,8 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
   const Across<T> wg{(const T*)a.wg, a.wgs, n * S::BN, a.K}, wu{(const T*)a.wu, a.wus, n * S::BN, a.K};
   const int f0 = blockIdx.y * a.xchunk, f1 = min(f0 + a.xchunk, a.F);
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(dg, wg, f0, f1, lds0, lds1, acc);
-  multiply<T, S, WIDE>(du, wu, f0, f1, lds0, lds1, acc);
+  multiply<T, S, WIDE>(dg, wg, f0, f1, lds, acc);
+  multiply<T, S, WIDE>(du, wu, f0, f1, lds, acc);
   const int rows = a.M - m * S::BM, cols = a.K - n * S::BN;
   if constexpr (sizeof(T) == 4)
     mend<S>(rows, [&](int c) { return c < cols; },
@@ -207,8 +227,8 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dx(GatedArgs a) {
 // parts of [dWg; dWu] = d^T x: split s takes the rows [s chunk, (s + 1) chunk). Where the
 // splits are a multiple of 8, the blocks of one run on one XCD, which then reads those rows of d and x from memory once.
 template <typename T, typename S, bool WIDE>
-__global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
-  __shared__ __align__(16) char lds0[Lds<T, S>::kA + Lds<T, S>::kB], lds1[Lds<T, S>::kA + Lds<T, S>::kB];
+__global__ __launch_bounds__(S::kThreads, S::BM == 256 ? 2 : 1) void k_gated_dw(GatedArgs a) {
+  G1NN_LDS(T, S, WIDE);
   const int tm = (2 * a.half + S::BM - 1) / S::BM, tn = (a.K + S::BN - 1) / S::BN;
   int split, t;
   if (a.splits % 8 == 0) {
@@ -223,7 +243,7 @@ __global__ __launch_bounds__(S::kThreads) void k_gated_dw(GatedArgs a) {
   const Across<T> B{(const T*)a.x, a.xs, n * S::BN, a.K};
   const long k0 = (long)split * a.chunk, end = k0 + a.chunk < a.M ? k0 + a.chunk : a.M;
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
-  multiply<T, S, WIDE>(A, B, k0, end, lds0, lds1, acc);
+  multiply<T, S, WIDE>(A, B, k0, end, lds, acc);
   const int rows = 2 * a.half - m * S::BM, cols = a.K - n * S::BN;
   if constexpr (sizeof(T) == 4)
     mend<S>(rows, [&](int c) { return c < cols; }, [&](int r, int c) { return again(A, r, B, c, k0, end); }, acc);
@@ -422,9 +442,6 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
-// Tiles of 128 x 128 where they give every CU one; else of 64 x 64, four times as many.
-inline bool large(long m, long n) { return ((m + 127) / 128) * ((n + 127) / 128) >= 256; }
-
 template <typename T, typename O, typename S, bool GRAD, int ACT>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
   const dim3 grid(tile_grid((a.M + S::BM - 1) / S::BM, ((GRAD ? a.half : a.F) + S::BN / 2 - 1) / (S::BN / 2)));
@@ -432,10 +449,21 @@ int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
   return launch(k_gated<T, O, S, false, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
 }
 
+// (the gradients' epilogue leaves no registers for a huge tile's accumulators)
+template <bool GRAD>
+Size gated_size(const GatedArgs& a) {
+  const Size s = size_of(a.M, 2l * a.F);
+  return GRAD && s == kHuge ? kLarge : s;
+}
+
 template <typename T, typename O, bool GRAD, int ACT>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
-  if (large(a.M, 2l * a.F)) return run_gated<T, O, Large, GRAD, ACT>(a, wide, st);
-  return run_gated<T, O, Small, GRAD, ACT>(a, wide, st);
+  const Size s = gated_size<GRAD>(a);
+  if constexpr (!GRAD) {
+    if (s == kHuge) return run_gated<T, O, typename Tiles<T>::Huge, GRAD, ACT>(a, wide, st);
+  }
+  if (s == kLarge) return run_gated<T, O, typename Tiles<T>::Large, GRAD, ACT>(a, wide, st);
+  return run_gated<T, O, typename Tiles<T>::Small, GRAD, ACT>(a, wide, st);
 }
 
 template <typename T, typename O, int ROWS, bool GRAD>
@@ -470,6 +498,13 @@ int run_dx(const GatedArgs& a, bool wide, hipStream_t st) {
   return launch(k_gated_dx<T, S, false>, grid, dim3(S::kThreads), st, a);
 }
 
+template <typename T>
+int run_dx(const GatedArgs& a, Size s, bool wide, hipStream_t st) {
+  if (s == kHuge) return run_dx<T, typename Tiles<T>::Huge>(a, wide, st);
+  if (s == kLarge) return run_dx<T, typename Tiles<T>::Large>(a, wide, st);
+  return run_dx<T, typename Tiles<T>::Small>(a, wide, st);
+}
+
 template <typename T, typename S>
 int run_dw(const GatedArgs& a, bool wide, hipStream_t st) {
   const dim3 grid((unsigned)(a.splits * ((2 * a.half + S::BM - 1) / S::BM) * (long)((a.K + S::BN - 1) / S::BN)));
@@ -477,25 +512,33 @@ int run_dw(const GatedArgs& a, bool wide, hipStream_t st) {
   return launch(k_gated_dw<T, S, false>, grid, dim3(S::kThreads), st, a);
 }
 
+template <typename T>
+int run_dw(const GatedArgs& a, Size s, bool wide, hipStream_t st) {
+  if (s == kHuge) return run_dw<T, typename Tiles<T>::Huge>(a, wide, st);
+  if (s == kLarge) return run_dw<T, typename Tiles<T>::Large>(a, wide, st);
+  return run_dw<T, typename Tiles<T>::Small>(a, wide, st);
+}
+
 // How the long sums are split. [dWg; dWu] over the rows: as many parts as give two blocks to each CU, of 256 rows at
 // least, and a multiple of eight (one L2 each) from three on. dx over the outputs, only where its tiles leave CUs idle:
 // parts of 128 outputs of both projections at least.
 struct Split {
   int half, splits, chunk, xsplits, xchunk;
-  bool large, xlarge;
+  Size w, x;
   Split(long M, int K, int F) {
     half = (F + 63) / 64 * 64;
-    const long t128 = ((2l * half + 127) / 128) * ((K + 127) / 128), t64 = (2l * half / 64) * ((K + 63) / 64);
-    large = t128 * ((M + 255) / 256) >= 512;
-    const long tiles = large ? t128 : t64, most = (M + 255) / 256;
+    const long most = (M + 255) / 256;
+    const long huge = ((2l * half + 255) / 256) * ((K + 127) / 128), big = ((2l * half + 127) / 128) * ((K + 127) / 128);
+    w = huge * most >= 2048 ? kHuge : big * most >= 512 ? kLarge : kSmall;
+    const long tiles = w == kHuge ? huge : w == kLarge ? big : (2l * half / 64) * ((K + 63) / 64);
     long s = (512 + tiles - 1) / tiles;
     if (s > 2) s = (s + 7) / 8 * 8;
     s = std::max(1l, std::min(s, most));
     chunk = (int)std::max(64l, ((M + s - 1) / s + 63) / 64 * 64);
     splits = (int)((M + chunk - 1) / chunk);
-    xlarge = g1nn::large(M, K);
-    const long x = xlarge ? 256 : ((M + 63) / 64) * ((K + 63) / 64);
-    s = x > 0 ? std::max(1l, std::min(256 / x, (F + 127l) / 128)) : 1;
+    x = size_of(M, K);
+    const long t = x != kSmall ? 256 : ((M + 63) / 64) * ((K + 63) / 64);
+    s = t > 0 ? std::max(1l, std::min(256 / t, (F + 127l) / 128)) : 1;
     xchunk = (int)(((F + s - 1) / s + 63) / 64 * 64);
     xsplits = (F + xchunk - 1) / xchunk;
   }
@@ -527,17 +570,20 @@ int gated_backward(GatedArgs a, const Split& s, hipStream_t st) {
   const bool wide = xw && even(a.wg, a.wgs, a.K, size, 16) && even(a.wu, a.wus, a.K, size, 16);
   const bool weights = a.dwg || a.dwu, biases = a.dbg || a.dbu;
   if (!biases) a.sums = nullptr;
-  const bool big = large(a.M, 2l * a.F);
-  a.sum_rows = a.M <= kFew ? 1 : big ? (a.M + Large::BM - 1) / Large::BM * Large::WM : (a.M + Small::BM - 1) / Small::BM * Small::WM;
+  using Large = typename Tiles<T>::Large;
+  using Small = typename Tiles<T>::Small;
+  a.sum_rows = a.M <= kFew                        ? 1
+               : gated_size<true>(a) == kLarge ? (a.M + Large::BM - 1) / Large::BM * Large::WM
+                                               : (a.M + Small::BM - 1) / Small::BM * Small::WM;
   if (a.M > 0) {
     int rc = run_gated<T, T, true>(a, wide, st);
     if (rc) return rc;
     if (a.dx) {
-      rc = s.xlarge ? run_dx<T, Large>(a, wide, st) : run_dx<T, Small>(a, wide, st);
+      rc = run_dx<T>(a, s.x, wide, st);
       if (rc) return rc;
     }
     if (weights) {
-      rc = s.large ? run_dw<T, Large>(a, xw, st) : run_dw<T, Small>(a, xw, st);
+      rc = run_dw<T>(a, s.w, xw, st);
       if (rc) return rc;
     }
   } else {

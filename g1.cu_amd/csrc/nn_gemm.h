@@ -337,31 +337,39 @@ struct Mma<i8> {
 };
 
 // A block's tile is BM x BN, on WM x WN waves of IM x JN accumulators of 32 x 32. Its depth in 16-byte chunks goes by type:
-// two chunks of fp32 planes, or four (DEEP); eight of bf16, four of int8.
-template <int BM_, int BN_, int WM_, int WN_, bool DEEP_>
+// DEPTH chunks of fp32 planes, of bf16 or of int8.
+template <int BM_, int BN_, int WM_, int WN_, int DEPTH_>
 struct Shape {
-  static constexpr bool DEEP = DEEP_;
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, DEPTH = DEPTH_;
   static constexpr int kThreads = WM * WN * 64, IM = BM / WM / 32, JN = BN / WN / 32;
 };
 
-template <typename T, typename S>
-constexpr int slots = sizeof(T) == 4 ? (S::DEEP ? 4 : 2) : sizeof(T) == 2 ? 8 : 4;
-
-// LDS of a block: two tiles of both operands
-template <typename T, typename S>
+// LDS of a block: tiles of both operands, two where they come through registers and three where they come directly. They
+// are separate arrays, so that the compiler knows reads of one from writes of another.
+template <typename T, typename S, bool WIDE>
 struct Lds {
-  static constexpr int kA = Form<T>::kPlanes * S::BM * slots<T, S> * 16, kB = Form<T>::kPlanes * S::BN * slots<T, S> * 16;
+  static constexpr bool kDirect = WIDE && sizeof(T) != 4;
+  static constexpr int kA = Form<T>::kPlanes * S::BM * S::DEPTH * 16, kB = Form<T>::kPlanes * S::BN * S::DEPTH * 16;
+  static constexpr int kTile = kA + kB, kThird = kDirect ? kTile : 16;
 };
+struct Tiles3 {
+  char *a, *b, *c;
+  __device__ __forceinline__ char* at(int i) const { return i == 0 ? a : i == 1 ? b : c; }
+};
+#define G1NN_LDS(T, S, WIDE)                                                           \
+  __shared__ __align__(16) char lds0[Lds<T, S, WIDE>::kTile], lds1[Lds<T, S, WIDE>::kTile], \
+      lds2[Lds<T, S, WIDE>::kThird];                                                   \
+  const Tiles3 lds{lds0, lds1, lds2}
 
-// The accumulators over k in [k0, end), with two LDS buffers and one barrier a tile. fp32: while a tile is multiplied,
-// the next one goes from registers into the other buffer (the splitting runs under the matrix instructions) and the one
-// after it is on its way from memory. bf16 and int8: while a tile is multiplied, the next one is on its way into the
-// other buffer.
+// The accumulators over k in [k0, end), with one barrier a tile. fp32: while a tile is multiplied, the next one goes from
+// registers into the other buffer (the splitting runs under the matrix instructions) and the one after it is on its way
+// from memory. bf16 and int8: while a tile is multiplied, the next two are on their way into the other buffers, and a
+// wave waits for its pieces of the nearer one only.
 template <typename T, typename S, bool WIDE, typename OpA, typename OpB>
 struct Product {
-  static constexpr int P = Form<T>::kPlanes, kSlots = slots<T, S>, D = kSlots * Form<T>::kPer;
-  static constexpr bool kDirect = WIDE && sizeof(T) != 4;
+  static constexpr int P = Form<T>::kPlanes, kSlots = S::DEPTH, D = kSlots * Form<T>::kPer;
+  static constexpr int kA = Lds<T, S, WIDE>::kA;
+  static constexpr bool kDirect = Lds<T, S, WIDE>::kDirect;
   typedef typename Mma<T>::Op Op;
   typedef typename Form<T>::Acc Acc;
   template <typename O, int ROWS>
@@ -394,7 +402,7 @@ struct Product {
 #pragma unroll
       for (int i = 0; i < S::IM; i++) a[p][i] = fragment<OpA, S::BM>(lds, p, ra + i * 32, s);
 #pragma unroll
-      for (int j = 0; j < S::JN; j++) b[p][j] = fragment<OpB, S::BN>(lds + Lds<T, S>::kA, p, rb + j * 32, s);
+      for (int j = 0; j < S::JN; j++) b[p][j] = fragment<OpB, S::BN>(lds + kA, p, rb + j * 32, s);
     }
     // the planes' products, the smallest first
     constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
@@ -409,19 +417,50 @@ struct Product {
 #pragma unroll
     for (int s = 0; s < kSlots / 2; s++) step(lds, s, acc);
   }
-  // every wave's reads of this tile, and its pieces of the next one, are done
-  static __device__ __forceinline__ void turn_over() {
-    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+  // Every wave's reads of the tile before, and its pieces of the next one, are done: at most `newer` pieces that were asked
+  // for later may still be on their way.
+  template <int NEWER>
+  static __device__ __forceinline__ void arrive() {
+    // the builtin, so that the compiler counts with it and adds no wait of its own: vmcnt(NEWER) and lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((NEWER & 15) | (NEWER >> 4 << 14) | 7 << 4);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
-
+  __device__ __forceinline__ void fetch(const OpA& A, const OpB& B, long k, char* lds) const {
+    sa.fetch(A, k, lds);
+    sb.fetch(B, k, lds + kA);
+    __builtin_amdgcn_sched_barrier(0);   // asked for before the products of the tile at hand
+  }
   __device__ __forceinline__ void fetch(const OpA& A, const OpB& B, long k, long end, char* lds) const {
     if (k + D <= end) {
-      sa.fetch(A, k, lds);
-      sb.fetch(B, k, lds + Lds<T, S>::kA);
+      fetch(A, B, k, lds);
     } else {
       sa.fetch(A, k, end, lds);
-      sb.fetch(B, k, end, lds + Lds<T, S>::kA);
+      sb.fetch(B, k, end, lds + kA);
+    }
+  }
+  __device__ __forceinline__ void run_direct(const OpA& A, const OpB& B, long k0, long end, const Tiles3& lds,
+                                             Acc (&acc)[S::IM][S::JN]) const {
+    constexpr int kPieces = decltype(sa)::kUnits + decltype(sb)::kUnits;   // of a tile
+    fetch(A, B, k0, end, lds.a);
+    if (k0 + D < end) fetch(A, B, k0 + D, end, lds.b);
+    for (; k0 + 5 * D <= end; k0 += 3 * D) {
+      arrive<kPieces>();
+      fetch(A, B, k0 + 2 * D, lds.c);
+      tile(lds.a, acc);
+      arrive<kPieces>();
+      fetch(A, B, k0 + 3 * D, lds.a);
+      tile(lds.b, acc);
+      arrive<kPieces>();
+      fetch(A, B, k0 + 4 * D, lds.b);
+      tile(lds.c, acc);
+    }
+    for (int t = 0; k0 < end; k0 += D, t = t == 2 ? 0 : t + 1) {
+      if (k0 + D < end) arrive<kPieces>();
+      else arrive<0>();
+      if (k0 + 2 * D < end) fetch(A, B, k0 + 2 * D, end, lds.at(t == 0 ? 2 : t - 1));
+      tile(lds.at(t), acc);
     }
   }
   __device__ __forceinline__ void load(const OpA& A, const OpB& B, long k, long end) {
@@ -435,69 +474,51 @@ struct Product {
   }
   __device__ __forceinline__ void store(char* lds) const {
     sa.store(lds);
-    sb.store(lds + Lds<T, S>::kA);
+    sb.store(lds + kA);
   }
 
-  __device__ __forceinline__ void run(const OpA& A, const OpB& B, long k0, long end, char* lds0, char* lds1,
+  __device__ __forceinline__ void run(const OpA& A, const OpB& B, long k0, long end, const Tiles3& lds,
                                       Acc (&acc)[S::IM][S::JN]) {
     if (k0 >= end) return;
     sa.init(A);
     sb.init(B);
     __syncthreads();   // an earlier product's reads
     if constexpr (kDirect) {
-      fetch(A, B, k0, end, lds0);
-      turn_over();
-      for (; k0 + 3 * D <= end; k0 += 2 * D) {
-        sa.fetch(A, k0 + D, lds1);
-        sb.fetch(B, k0 + D, lds1 + Lds<T, S>::kA);
-        __builtin_amdgcn_sched_barrier(0);   // on their way first
-        tile(lds0, acc);
-        turn_over();
-        sa.fetch(A, k0 + 2 * D, lds0);
-        sb.fetch(B, k0 + 2 * D, lds0 + Lds<T, S>::kA);
-        __builtin_amdgcn_sched_barrier(0);   // on their way first
-        tile(lds1, acc);
-        turn_over();
-      }
-      for (int odd = 0; k0 < end; k0 += D, odd ^= 1) {
-        if (k0 + D < end) fetch(A, B, k0 + D, end, odd ? lds0 : lds1);
-        tile(odd ? lds1 : lds0, acc);
-        turn_over();
-      }
+      run_direct(A, B, k0, end, lds, acc);
     } else {
       load(A, B, k0, end);
-      store(lds0);
+      store(lds.a);
       if (k0 + D < end) load(A, B, k0 + D, end);
-      turn_over();
+      __syncthreads();
       for (; k0 + 4 * D <= end; k0 += 2 * D) {
-        store(lds1);
+        store(lds.b);
         sa.load(A, k0 + 2 * D);
         sb.load(B, k0 + 2 * D);
-        tile(lds0, acc);
-        turn_over();
-        store(lds0);
+        tile(lds.a, acc);
+        __syncthreads();
+        store(lds.a);
         sa.load(A, k0 + 3 * D);
         sb.load(B, k0 + 3 * D);
-        tile(lds1, acc);
-        turn_over();
+        tile(lds.b, acc);
+        __syncthreads();
       }
       for (int odd = 0; k0 < end; k0 += D, odd ^= 1) {
         if (k0 + D < end) {
-          store(odd ? lds0 : lds1);
+          store(lds.at(odd ^ 1));
           if (k0 + 2 * D < end) load(A, B, k0 + 2 * D, end);
         }
-        tile(odd ? lds1 : lds0, acc);
-        turn_over();
+        tile(lds.at(odd), acc);
+        __syncthreads();
       }
     }
   }
 };
 
 template <typename T, typename S, bool WIDE, typename OpA, typename OpB>
-__device__ __forceinline__ void multiply(const OpA& A, const OpB& B, long k0, long end, char* lds0, char* lds1,
+__device__ __forceinline__ void multiply(const OpA& A, const OpB& B, long k0, long end, const Tiles3& lds,
                                          typename Form<T>::Acc (&acc)[S::IM][S::JN]) {
   Product<T, S, WIDE, OpA, OpB> p;
-  p.run(A, B, k0, end, lds0, lds1, acc);
+  p.run(A, B, k0, end, lds, acc);
 }
 
 // One output again, in plain fp32
