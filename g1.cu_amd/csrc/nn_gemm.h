@@ -565,11 +565,18 @@ __device__ __forceinline__ void mend(int rows, C stored, V value, f32x16 (&acc)[
 }
 
 // Blocks to tiles (`tm` rows of `tn` tiles). Block b runs on XCD b mod 8; where there are enough rows of tiles for the eight
-// to share them evenly, a row stays on one XCD, so that its part of A is read from memory by one L2 only.
+// to share them evenly, a row stays on one XCD, so that its part of A is read from memory by one L2 only. An XCD goes
+// through eight rows at a time, column by column: its running blocks then share a few rows of both operands, which fit
+// its L2 beside the outputs.
 __device__ __forceinline__ bool tile_of(int b, int tm, int tn, int& m, int& n) {
-  const int i = tm >= 64 ? b >> 3 : b;
-  m = tm >= 64 ? i / tn * 8 + (b & 7) : i / tn;
-  n = i % tn;
+  if (tm < 64) {
+    m = b / tn;
+    n = b % tn;
+    return true;
+  }
+  const int each = (tm + 7) >> 3, i = b >> 3, first = i / (8 * tn) * 8, rows = min(8, each - first), j = i - first * tn;
+  m = (first + j % rows) * 8 + (b & 7);
+  n = j / rows;
   return m < tm;
 }
 inline unsigned tile_grid(long tm, long tn) { return (unsigned)((tm >= 64 ? (tm + 7) / 8 * 8 : tm) * tn); }
