@@ -71,19 +71,19 @@ struct GatedArgs {
   const float *s, *sg, *su;
 };
 
-// Tiles of a block by type, four chunks deep; in fp32 two chunks of three planes, and four where a block is small and waits
-// more.
+// Tiles of a block by type, four chunks deep, and eight where a block is small and waits more; in fp32 (three planes) half
+// of that.
 template <typename T>
 struct Tiles {
   using Huge = Shape<256, 128, 2, 2, 4>;
   using Large = Shape<128, 128, 2, 2, 4>;
-  using Small = Shape<64, 64, 2, 1, 4>;
+  using Small = Shape<64, 64, 2, 1, 8, 2>;
 };
 template <>
 struct Tiles<float> {
   using Huge = Shape<128, 128, 2, 2, 2>;
   using Large = Huge;
-  using Small = Shape<64, 64, 2, 1, 4>;
+  using Small = Shape<64, 64, 2, 1, 4, 2>;
 };
 
 // Which of them a product of m x n takes: the large ones where they give every CU a block, the huge ones (which read
@@ -163,7 +163,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
       if (a.sums) {
         sum_g += __shfl_xor(sum_g, 32);
         sum_u += __shfl_xor(sum_u, 32);
-        float* at = a.sums + ((long)m * S::WM + (threadIdx.x >> 6) / S::WN) * (2 * a.half) + f;
+        float* at = a.sums + ((long)m * S::WM + S::wave() / S::WN) * (2 * a.half) + f;
         if (lane < 32) {
           at[0] = sum_g;
           at[a.half] = sum_u;
@@ -174,7 +174,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
 }
 
 template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
-__global__ __launch_bounds__(S::kThreads, S::kThreads == 128 ? 1 : sizeof(T) == 4 ? 3 : 2) void k_gated(GatedArgs a) {
+__global__ __launch_bounds__(S::kThreads, S::KS == 2 ? 1 : sizeof(T) == 4 ? 3 : 2) void k_gated(GatedArgs a) {
   G1NN_LDS(T, S, WIDE);
   const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
   int m, n;
@@ -184,6 +184,8 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 128 ? 1 : sizeof(T) == 
   const Paired<T> B{(const T*)a.wg, (const T*)a.wu, a.wgs, a.wus, f0, a.F};
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
   multiply<T, S, WIDE>(A, B, 0, a.K, lds, acc);
+  gather<T, S>(lds, acc);
+  if (!S::outputs()) return;
   if constexpr (sizeof(T) == 4)
     mend<S>(a.M - m * S::BM, [&](int c) { return f0 + (c >> 6) * 32 + (c & 31) < a.F; },
             [&](int r, int c) { return again(A, r, B, c, 0, a.K); }, acc);
@@ -204,6 +206,8 @@ __global__ __launch_bounds__(S::kThreads, S::BM == 256 ? 2 : 1) void k_gated_dx(
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
   multiply<T, S, WIDE>(dg, wg, f0, f1, lds, acc);
   multiply<T, S, WIDE>(du, wu, f0, f1, lds, acc);
+  gather<T, S>(lds, acc);
+  if (!S::outputs()) return;
   const int rows = a.M - m * S::BM, cols = a.K - n * S::BN;
   if constexpr (sizeof(T) == 4)
     mend<S>(rows, [&](int c) { return c < cols; },
@@ -244,6 +248,8 @@ __global__ __launch_bounds__(S::kThreads, S::BM == 256 ? 2 : 1) void k_gated_dw(
   const long k0 = (long)split * a.chunk, end = k0 + a.chunk < a.M ? k0 + a.chunk : a.M;
   typename Form<T>::Acc acc[S::IM][S::JN] = {};
   multiply<T, S, WIDE>(A, B, k0, end, lds, acc);
+  gather<T, S>(lds, acc);
+  if (!S::outputs()) return;
   const int rows = 2 * a.half - m * S::BM, cols = a.K - n * S::BN;
   if constexpr (sizeof(T) == 4)
     mend<S>(rows, [&](int c) { return c < cols; }, [&](int r, int c) { return again(A, r, B, c, k0, end); }, acc);

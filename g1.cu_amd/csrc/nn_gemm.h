@@ -159,6 +159,14 @@ struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, true> {
     for (int i = 0; i < kUnits; i++) {
       const T* p = base(o, i) + k0 + off[i];
       const int n = (int)(end - k0) - unit(i) % SLOTS * kPer;
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int a = 0; a < kAcc; a++) {
+          v[i][a] = i32x4{0, 0, 0, 0};
+          if (a * 16 / (int)sizeof(T) < n) v[i][a] = reinterpret_cast<const i32x4*>(p)[a];
+        }
+        continue;
+      }
       constexpr int kIn = 4 / sizeof(T);   // elements of a word
 #pragma unroll
       for (int w = 0; w < kPer / kIn; w++) {
@@ -226,6 +234,11 @@ struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, false> {
       for (int l = 0; l < 4; l++) {
         const T* p = o.p + (k0 + l) * o.stride + off[i];
         const bool ok = k0 + unit(i) / kWidth * 4 + l < end;
+        if constexpr (WIDE) {
+          v[i][l] = u32x2{0, 0};
+          if (ok) v[i][l] = *reinterpret_cast<const u32x2*>(p);
+          continue;
+        }
         unsigned w[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < kCols; e++)
@@ -336,12 +349,18 @@ struct Mma<i8> {
   }
 };
 
-// A block's tile is BM x BN, on WM x WN waves of IM x JN accumulators of 32 x 32. Its depth in 16-byte chunks goes by type:
-// DEPTH chunks of fp32 planes, of bf16 or of int8.
-template <int BM_, int BN_, int WM_, int WN_, int DEPTH_>
+// A block's tile is BM x BN, on WM x WN waves of IM x JN accumulators of 32 x 32, DEPTH 16-byte chunks of k deep. With KS = 2
+// there are two such sets of waves, each of which multiplies every other step of a tile; the second one's sums go to
+// the first through LDS at the end. Small tiles take it: alone on a CU, half of the work between two barriers takes half
+// of the time.
+template <int BM_, int BN_, int WM_, int WN_, int DEPTH_, int KS_ = 1>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, DEPTH = DEPTH_;
-  static constexpr int kThreads = WM * WN * 64, IM = BM / WM / 32, JN = BN / WN / 32;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, DEPTH = DEPTH_, KS = KS_;
+  static constexpr int kSet = WM * WN, kThreads = kSet * KS * 64, IM = BM / WM / 32, JN = BN / WN / 32;
+  // the wave's place in its set
+  static __device__ __forceinline__ int wave() { return (threadIdx.x >> 6) % kSet; }
+  // whether the thread has outputs
+  static __device__ __forceinline__ bool outputs() { return KS == 1 || threadIdx.x < kSet * 64; }
 };
 
 // LDS of a block: tiles of both operands, two where they come through registers and three where they come directly. They
@@ -395,7 +414,7 @@ struct Product {
     }
   }
   static __device__ __forceinline__ void step(const char* lds, int s, Acc (&acc)[S::IM][S::JN]) {
-    const int wave = threadIdx.x >> 6, ra = wave / S::WN * S::IM * 32, rb = wave % S::WN * S::JN * 32;
+    const int wave = S::wave(), ra = wave / S::WN * S::IM * 32, rb = wave % S::WN * S::JN * 32;
     Op a[P][S::IM], b[P][S::JN];
 #pragma unroll
     for (int p = 0; p < P; p++) {
@@ -415,7 +434,7 @@ struct Product {
   }
   static __device__ __forceinline__ void tile(const char* lds, Acc (&acc)[S::IM][S::JN]) {
 #pragma unroll
-    for (int s = 0; s < kSlots / 2; s++) step(lds, s, acc);
+    for (int s = 0; s < kSlots / 2; s += S::KS) step(lds, s + (S::KS > 1 ? (int)(threadIdx.x >> 6) / S::kSet : 0), acc);
   }
   // Every wave's reads of the tile before, and its pieces of the next one, are done: at most `newer` pieces that were asked
   // for later may still be on their way.
@@ -486,9 +505,12 @@ struct Product {
     if constexpr (kDirect) {
       run_direct(A, B, k0, end, lds, acc);
     } else {
-      load(A, B, k0, end);
-      store(lds.a);
-      if (k0 + D < end) load(A, B, k0 + D, end);
+      {
+        Product first = *this;   // its registers, so that the first two tiles are on their way together
+        first.load(A, B, k0, end);
+        if (k0 + D < end) load(A, B, k0 + D, end);
+        first.store(lds.a);
+      }
       __syncthreads();
       for (; k0 + 4 * D <= end; k0 += 2 * D) {
         store(lds.b);
@@ -521,6 +543,32 @@ __device__ __forceinline__ void multiply(const OpA& A, const OpB& B, long k0, lo
   p.run(A, B, k0, end, lds, acc);
 }
 
+// With two sets of waves: the second one's sums added to the first one's.
+template <typename T, typename S, typename Acc>
+__device__ __forceinline__ void gather(const Tiles3& lds, Acc (&acc)[S::IM][S::JN]) {
+  if constexpr (S::KS == 2) {
+    static_assert(S::kSet * 64 * S::IM * S::JN * 16 * 4 <= (S::BM + S::BN) * S::DEPTH * 16 * (sizeof(T) == 4 ? 3 : 1), "one tile's LDS");
+    typedef decltype(acc[0][0][0] + acc[0][0][0]) V;
+    __syncthreads();
+    V* to = reinterpret_cast<V*>(lds.a) + threadIdx.x % (S::kSet * 64);
+#pragma unroll
+    for (int i = 0; i < S::IM; i++)
+#pragma unroll
+      for (int j = 0; j < S::JN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (!S::outputs()) to[((i * S::JN + j) * 16 + r) * S::kSet * 64] = acc[i][j][r];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::IM; i++)
+#pragma unroll
+      for (int j = 0; j < S::JN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (S::outputs()) acc[i][j][r] += to[((i * S::JN + j) * 16 + r) * S::kSet * 64];
+  }
+}
+
 // One output again, in plain fp32
 template <typename OpA, typename OpB>
 __device__ __attribute__((noinline)) float again(const OpA& A, int ra, const OpB& B, int rb, long k0, long end) {
@@ -532,13 +580,13 @@ __device__ __attribute__((noinline)) float again(const OpA& A, int ra, const OpB
 // row of C (within the block's tile) that register r of accumulator i holds
 template <typename S>
 __device__ __forceinline__ int c_row(int i, int r) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = S::wave();
   return wave / S::WN * S::IM * 32 + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
 }
 // and the column of accumulator j
 template <typename S>
 __device__ __forceinline__ int c_col(int j) {
-  return (int)(threadIdx.x >> 6) % S::WN * S::JN * 32 + j * 32 + (threadIdx.x & 31);
+  return S::wave() % S::WN * S::JN * 32 + j * 32 + (threadIdx.x & 31);
 }
 
 // The fp32 outputs that came out infinite or NaN, again: those of rows below `rows` and of columns that are stored
