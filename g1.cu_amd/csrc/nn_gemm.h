@@ -569,10 +569,11 @@ __device__ __forceinline__ void gather(const Tiles3& lds, Acc (&acc)[S::IM][S::J
   }
 }
 
-// One output again, in plain fp32
+// One output again, in plain fp32. (Not a function of its own: a call would give every wave of the kernel a stack.)
 template <typename OpA, typename OpB>
-__device__ __attribute__((noinline)) float again(const OpA& A, int ra, const OpB& B, int rb, long k0, long end) {
+__device__ __forceinline__ float again(const OpA& A, int ra, const OpB& B, int rb, long k0, long end) {
   float v = 0;
+#pragma unroll 1
   for (long k = k0; k < end; k++) v = __builtin_fmaf((float)A.at(ra, k), (float)B.at(rb, k), v);
   return v;
 }
@@ -600,7 +601,7 @@ __device__ __forceinline__ void mend(int rows, C stored, V value, f32x16 (&acc)[
     for (int j = 0; j < S::JN; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) z = __builtin_fmaf(acc[i][j][r], 0.0f, z);
-  if (z == 0) return;
+  if (__builtin_expect(z == 0, 1)) return;
 #pragma unroll
   for (int i = 0; i < S::IM; i++)
 #pragma unroll
