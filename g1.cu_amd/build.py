@@ -11,6 +11,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT_DIR = os.path.join(HERE, "build")
@@ -87,6 +88,21 @@ def _compile(name, extra):
     return obj, cmd, p
 
 
+def build_torch_module():
+    """g1nn_torch, the Python extension module around the policy operators' C entries: host code alone, against torch's
+    headers and libg1env.so, which lies beside it."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    out = os.path.join(OUT_DIR, "g1nn_torch.so")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root}/include",
+           f"-I{root}/include/torch/csrc/api/include", "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}",
+           os.path.join(HERE, "csrc", "nn_torch.cpp"), "-o", out + ".tmp", f"-L{root}/lib", f"-L{OUT_DIR}", "-lc10",
+           "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-l:libg1env.so", "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True)
+    os.replace(out + ".tmp", out)
+
+
 def build(verbose=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     objs = []
@@ -107,6 +123,7 @@ def build(verbose=False):
     for obj in objs:
         os.remove(obj)
     os.replace(OUT + ".tmp", OUT)
+    build_torch_module()
     with open(RESOURCES, "w") as f:
         json.dump(resources, f, indent=1, sort_keys=True)
     for fn, r in resources.items():

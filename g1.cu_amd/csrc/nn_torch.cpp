@@ -1,0 +1,400 @@
+// nn_torch.cpp -- the policy operators on torch tensors: checks, outputs and workspaces from torch's allocator, its
+// current stream, and the autograd nodes, around the C entries of g1nn.h. A Python extension module of its own
+// (g1nn_torch), which g1nn.py wraps; in C++ because a call of a small operator costs more on the host than on the GPU
+// (one gated block of one row: 9.4 us of host time from Python over ctypes, of which 3.6 are the launch).
+//
+// A tensor that a kernel does not take raises ValueError, a failed launch RuntimeError.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "../../include/g1nn.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int type_of(at::ScalarType t, const char* name) {
+  TORCH_CHECK_VALUE(t == at::kFloat || t == at::kBFloat16, name, " is ", t, ": float32 and bfloat16 are supported");
+  return t == at::kFloat ? 0 : 1;
+}
+
+// The tensor that the others have to go with: its type code.
+int first(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.defined() && x.is_cuda(), name, " is not a tensor on a GPU");
+  const int code = type_of(x.scalar_type(), name);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, name, " has no row elements");
+  return code;
+}
+
+void want(const Tensor& t, const char* name, const Tensor& like, at::ScalarType type) {
+  TORCH_CHECK_VALUE(t.defined(), name, " is not a tensor");
+  TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", not on ", like.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == type, name, " is ", t.scalar_type(), ", not ", type);
+}
+
+void shaped(const Tensor& t, const char* name, at::IntArrayRef sizes) {
+  TORCH_CHECK_VALUE(t.sizes() == sizes, name, " has shape ", t.sizes(), ", not ", sizes);
+}
+
+// Address of a contiguous tensor of that shape; null for none.
+void* whole(const Tensor& t, const char* name, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes) {
+  if (!t.defined()) return nullptr;
+  want(t, name, like, type);
+  shaped(t, name, sizes);
+  TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+  return t.data_ptr();
+}
+
+bool even(const Tensor& t) { return t.is_contiguous() || (t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1)); }
+
+// Elements from row to row of t seen as rows of its last dimension.
+long stride(const Tensor& t, const char* name) {
+  if (t.is_contiguous()) return t.size(-1);
+  TORCH_CHECK_VALUE(even(t), name, ": rows must be contiguous, and evenly spaced");
+  return t.stride(0);
+}
+
+// Gradients come in any layout.
+Tensor evened(const Tensor& t) { return even(t) ? t : t.contiguous(); }
+
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
+Tensor bytes(long n, const Tensor& t) { return at::empty({n}, t.options().dtype(at::kByte)); }
+
+// The place of a call: its device is current while it lives, and `stream` the current stream there.
+struct Place {
+  c10::DeviceGuard guard;
+  void* stream;
+  explicit Place(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
+
+void done(int rc) {
+  if (rc == 0) return;
+  TORCH_CHECK_VALUE(rc != -1, "refused by libg1env.so (the reason is on stderr)");
+  TORCH_CHECK(false, "a kernel launch failed (the reason is on stderr)");
+}
+
+void once() {
+  // in a backward pass, gradients are enabled only where a graph of it is asked for
+  TORCH_CHECK(!at::GradMode::is_enabled(), "the gradients of g1nn's operators cannot be differentiated again (create_graph)");
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// ---- norm ---------------------------------------------------------------------------------------------------------
+struct Normed {
+  Tensor y, h, last;   // last: rstd, or the scales of 8-bit rows
+};
+
+Normed norm(const Tensor& x, const Tensor& w, const Tensor& r, double eps, bool q8, bool keep) {
+  const int code = first(x, "x");
+  const long K = x.size(-1), M = x.numel() / K;
+  TORCH_CHECK_VALUE(w.defined(), "weight is not a tensor");
+  const void* wp = whole(w, "weight", x, x.scalar_type(), {K});
+  const long xs = stride(x, "x");
+  long rs = 0;
+  if (r.defined()) {
+    want(r, "residual", x, x.scalar_type());
+    shaped(r, "residual", x.sizes());
+    rs = stride(r, "residual");
+  }
+  const Place at(x);
+  Normed o;
+  o.y = q8 ? at::empty(x.sizes(), x.options().dtype(at::kChar)) : like(x);
+  if (r.defined()) o.h = like(x);
+  if (q8) o.last = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  else if (keep) o.last = at::empty({M}, x.options().dtype(at::kFloat));
+  if (q8)
+    done(g1_nn_rms_norm_q8(code, M, (int)K, x.data_ptr(), xs, address(r), rs, wp, (float)eps, (signed char*)o.y.data_ptr(),
+                           (float*)o.last.data_ptr(), address(o.h), at.stream));
+  else
+    done(g1_nn_rms_norm(code, M, (int)K, x.data_ptr(), xs, address(r), rs, wp, (float)eps, o.y.data_ptr(), address(o.h),
+                        (float*)address(o.last), at.stream));
+  return o;
+}
+
+struct NormNode : torch::autograd::Function<NormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& r,
+                               double eps) {
+    ctx->set_materialize_grads(false);
+    Normed o = norm(x, w, r.value_or(Tensor()), eps, false, true);
+    ctx->saved_data["stream"] = r.has_value();
+    ctx->save_for_backward({r ? o.h : x, o.last, w});
+    if (!r) return {o.y};
+    return {o.y, o.h};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &rstd = saved[1], &w = saved[2];
+    Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+    const bool stream = ctx->saved_data["stream"].toBool();   // the residual has a gradient of its own
+    if (!dy.defined()) return {dh, Tensor(), stream ? dh : Tensor(), Tensor()};
+    dy = evened(dy);
+    if (dh.defined()) dh = evened(dh);
+    const int code = type_of(h.scalar_type(), "h");
+    const long K = h.size(-1), M = h.numel() / K;
+    const Place at(h);
+    Tensor dx = like(h), dw, ws;
+    if (ctx->needs_input_grad(1)) {
+      dw = like(w);
+      ws = bytes(g1_nn_rms_norm_backward_workspace(code, M, (int)K), h);
+    }
+    done(g1_nn_rms_norm_backward(code, M, (int)K, dy.data_ptr(), stride(dy, "dy"), address(dh),
+                                 dh.defined() ? stride(dh, "dh") : 0, h.data_ptr(), stride(h, "h"),
+                                 (const float*)rstd.data_ptr(), w.data_ptr(), dx.data_ptr(), address(dw), address(ws),
+                                 at.stream));
+    return {dx, dw, stream ? dx : Tensor(), Tensor()};
+  }
+};
+
+// ---- gated block --------------------------------------------------------------------------------------------------
+struct Gated {
+  int code;
+  long M, xs, wgs, wus;
+  int K, F;
+  const void *x, *wg, *wu, *bg, *bu;
+  Gated(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& bg_, const Tensor& bu_) {
+    code = first(x_, "x");
+    const auto type = x_.scalar_type();
+    const long k = x_.size(-1);
+    want(wg_, "w_gate", x_, type);
+    TORCH_CHECK_VALUE(wg_.dim() == 2 && wg_.size(0) >= 1 && wg_.size(1) == k, "w_gate has shape ", wg_.sizes(), ", not (F, ", k,
+                      ")");
+    want(wu_, "w_up", x_, type);
+    shaped(wu_, "w_up", wg_.sizes());
+    const long f = wg_.size(0);
+    TORCH_CHECK_VALUE(k <= 131072 && f <= 131072, "widths of 1 to 131072 are supported");
+    M = x_.numel() / k, K = (int)k, F = (int)f;
+    xs = stride(x_, "x"), wgs = stride(wg_, "w_gate"), wus = stride(wu_, "w_up");
+    bg = whole(bg_, "b_gate", x_, type, {f}), bu = whole(bu_, "b_up", x_, type, {f});
+    x = x_.data_ptr(), wg = wg_.data_ptr(), wu = wu_.data_ptr();
+  }
+};
+
+Tensor rows_of(const Tensor& x, long F, at::ScalarType type) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = F;
+  return at::empty(sizes, x.options().dtype(type));
+}
+
+Tensor gated(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu, int act) {
+  const Gated g(x, wg, wu, bg, bu);
+  const Place at(x);
+  Tensor y = rows_of(x, g.F, x.scalar_type());
+  done(g1_nn_gated(g.code, g.M, g.K, g.F, g.x, g.xs, g.wg, g.wgs, g.wu, g.wus, g.bg, g.bu, act, y.data_ptr(), at.stream));
+  return y;
+}
+
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
+                        const std::optional<Tensor>& bg, const std::optional<Tensor>& bu, int64_t act) {
+    ctx->saved_data["act"] = act;
+    const Tensor a = bg.value_or(Tensor()), b = bu.value_or(Tensor());
+    ctx->save_for_backward({x, wg, wu, a, b});
+    return gated(x, wg, wu, a, b, (int)act);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    const variable_list saved = ctx->get_saved_variables();
+    const Gated g(saved[0], saved[1], saved[2], saved[3], saved[4]);
+    const Tensor dy = evened(grads[0]);
+    const Place at(dy);
+    variable_list out(6);
+    // the node counts the tensors that were given
+    for (int i = 0, edge = 0; i < 5; i++)
+      if (saved[i].defined() && ctx->needs_input_grad(edge++)) out[i] = like(saved[i]);
+    const Tensor ws = bytes(g1_nn_gated_backward_workspace(g.code, g.M, g.K, g.F), dy);
+    done(g1_nn_gated_backward(g.code, g.M, g.K, g.F, g.x, g.xs, g.wg, g.wgs, g.wu, g.wus, g.bg, g.bu,
+                              (int)ctx->saved_data["act"].toInt(), dy.data_ptr(), stride(dy, "dy"), address(out[0]),
+                              address(out[1]), address(out[2]), address(out[3]), address(out[4]), ws.data_ptr(), at.stream));
+    return out;
+  }
+};
+
+Tensor gated_q8(const Tensor& q, const Tensor& s, const Tensor& qg, const Tensor& sg, const Tensor& qu, const Tensor& su,
+                const Tensor& bg, const Tensor& bu, int act, at::ScalarType type) {
+  TORCH_CHECK_VALUE(q.defined() && q.is_cuda() && q.scalar_type() == at::kChar && q.dim() >= 1 && q.size(-1) >= 1,
+                    "q is not an int8 tensor of rows on a GPU");
+  const int code = type_of(type, "dtype");
+  const long k = q.size(-1);
+  want(qg, "w_gate_q", q, at::kChar);
+  TORCH_CHECK_VALUE(qg.dim() == 2 && qg.size(0) >= 1 && qg.size(1) == k, "w_gate_q has shape ", qg.sizes(), ", not (F, ", k,
+                    ")");
+  const long f = qg.size(0);
+  TORCH_CHECK_VALUE(k <= 131072 && f <= 131072, "widths of 1 to 131072 are supported");
+  TORCH_CHECK_VALUE(s.defined() && sg.defined() && qu.defined() && su.defined(), "scale, s_gate, w_up_q or s_up is not a tensor");
+  const auto* sp = (const float*)whole(s, "scale", q, at::kFloat, q.sizes().slice(0, q.dim() - 1));
+  const auto* gp = (const signed char*)whole(qg, "w_gate_q", q, at::kChar, qg.sizes());
+  const auto* sgp = (const float*)whole(sg, "s_gate", q, at::kFloat, {f});
+  const auto* up = (const signed char*)whole(qu, "w_up_q", q, at::kChar, qg.sizes());
+  const auto* sup = (const float*)whole(su, "s_up", q, at::kFloat, {f});
+  const auto* bgp = (const float*)whole(bg, "b_gate", q, at::kFloat, {f});
+  const auto* bup = (const float*)whole(bu, "b_up", q, at::kFloat, {f});
+  const long qs = stride(q, "q");
+  const Place at(q);
+  Tensor y = rows_of(q, f, type);
+  done(g1_nn_gated_q8(code, q.numel() / k, (int)k, (int)f, (const signed char*)q.data_ptr(), qs, sp, gp, sgp, up, sup, bgp,
+                      bup, act, y.data_ptr(), at.stream));
+  return y;
+}
+
+// ---- clipping -----------------------------------------------------------------------------------------------------
+struct Tensors {
+  std::vector<Tensor> t;
+  std::vector<void*> at;
+  std::vector<int> type;
+  Tensors(PyObject* seq, const char* what) {
+    THPObjectPtr fast(PySequence_Fast(seq, "a sequence of tensors"));
+    if (!fast) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.get());
+    t.reserve(n), at.reserve(n), type.reserve(n);
+    for (Py_ssize_t i = 0; i < n; i++) {
+      PyObject* o = PySequence_Fast_GET_ITEM(fast.get(), i);
+      TORCH_CHECK_VALUE(THPVariable_Check(o), what, " is not a tensor");
+      t.push_back(THPVariable_Unpack(o));
+      const Tensor& x = t.back();
+      TORCH_CHECK_VALUE(x.is_cuda() && x.device() == t[0].device(), what, " is on ", x.device(),
+                        ": all are on one GPU");
+      type.push_back(type_of(x.scalar_type(), what));
+      TORCH_CHECK_VALUE(x.is_contiguous(), what, " is not contiguous");
+      at.push_back(x.data_ptr());
+    }
+  }
+};
+
+Tensor clip(PyObject* grads, double max_norm, PyObject* out) {
+  const Tensors in(grads, "a gradient");
+  const int n = (int)in.t.size();
+  TORCH_CHECK_VALUE(n > 0, "no gradients");
+  std::optional<Tensors> to;
+  if (out != Py_None) {
+    to.emplace(out, "an output");
+    TORCH_CHECK_VALUE(to->t.size() == in.t.size(), n, " gradients and ", to->t.size(), " outputs");
+    TORCH_CHECK_VALUE(to->t[0].device() == in.t[0].device(), "the outputs are not on the gradients' GPU");
+    for (int i = 0; i < n; i++) shaped(to->t[i], "an output", in.t[i].sizes());
+  }
+  const Tensors& o = to ? *to : in;
+  std::vector<long> size(n);
+  for (int i = 0; i < n; i++) size[i] = in.t[i].numel();
+  const Place at(in.t[0]);
+  Tensor norm = at::empty({}, in.t[0].options().dtype(at::kFloat));
+  const Tensor ws = bytes(g1_nn_clip_workspace(n), in.t[0]);
+  done(g1_nn_clip(n, in.at.data(), in.type.data(), o.at.data(), o.type.data(), size.data(), (float)max_norm,
+                  (float*)norm.data_ptr(), ws.data_ptr(), at.stream));
+  for (const Tensor& t : o.t)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // written in place
+  return norm;
+}
+
+// ---- the module ---------------------------------------------------------------------------------------------------
+Tensor tensor(PyObject* o, const char* name) {
+  TORCH_CHECK_VALUE(THPVariable_Check(o), name, " is not a tensor");
+  return THPVariable_Unpack(o);
+}
+Tensor maybe(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor(o, name); }
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
+PyObject* wrap(const std::vector<Tensor>& ts) {
+  THPObjectPtr tuple(PyTuple_New((Py_ssize_t)ts.size()));
+  if (!tuple) throw python_error();
+  for (size_t i = 0; i < ts.size(); i++) PyTuple_SET_ITEM(tuple.get(), (Py_ssize_t)i, wrap(ts[i]));
+  return tuple.release();
+}
+
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+bool takes(Py_ssize_t have, Py_ssize_t want) {
+  if (have == want) return true;
+  PyErr_Format(PyExc_TypeError, "%zd arguments, not %zd", have, want);
+  return false;
+}
+
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 4)) return nullptr;
+  const Tensor x = tensor(a[0], "x"), w = tensor(a[1], "weight"), r = maybe(a[2], "residual");
+  const double eps = number(a[3]);
+  if (wants_grad({&x, &w, &r})) {
+    const variable_list o = NormNode::apply(x, w, given(r), eps);
+    return r.defined() ? wrap(o) : wrap(o[0]);
+  }
+  const Normed o = norm(x, w, r, eps, false, false);
+  return r.defined() ? wrap(std::vector<Tensor>{o.y, o.h}) : wrap(o.y);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 4)) return nullptr;
+  const Normed o = norm(tensor(a[0], "x"), tensor(a[1], "weight"), maybe(a[2], "residual"), number(a[3]), true, false);
+  return o.h.defined() ? wrap(std::vector<Tensor>{o.y, o.last, o.h}) : wrap(std::vector<Tensor>{o.y, o.last});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_gated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 6)) return nullptr;
+  const Tensor x = tensor(a[0], "x"), wg = tensor(a[1], "w_gate"), wu = tensor(a[2], "w_up"), bg = maybe(a[3], "b_gate"),
+               bu = maybe(a[4], "b_up");
+  const long act = (long)number(a[5]);
+  if (wants_grad({&x, &wg, &wu, &bg, &bu})) return wrap(GatedNode::apply(x, wg, wu, given(bg), given(bu), (int64_t)act));
+  return wrap(gated(x, wg, wu, bg, bu, (int)act));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_gated_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 10)) return nullptr;
+  return wrap(gated_q8(tensor(a[0], "q"), tensor(a[1], "scale"), tensor(a[2], "w_gate_q"), tensor(a[3], "s_gate"),
+                       tensor(a[4], "w_up_q"), tensor(a[5], "s_up"), maybe(a[6], "b_gate"), maybe(a[7], "b_up"),
+                       (int)number(a[8]), PyObject_IsTrue(a[9]) ? at::kBFloat16 : at::kFloat));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 3)) return nullptr;
+  return wrap(clip(a[0], number(a[1]), a[2]));
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef kMethods[] = {
+    {"rms_norm", (PyCFunction)(void*)py_rms_norm, METH_FASTCALL, "(x, weight, residual, eps)"},
+    {"rms_norm_q8", (PyCFunction)(void*)py_rms_norm_q8, METH_FASTCALL, "(x, weight, residual, eps)"},
+    {"gated", (PyCFunction)(void*)py_gated, METH_FASTCALL, "(x, w_gate, w_up, b_gate, b_up, activation)"},
+    {"gated_q8", (PyCFunction)(void*)py_gated_q8, METH_FASTCALL,
+     "(q, scale, w_gate_q, s_gate, w_up_q, s_up, b_gate, b_up, activation, bf16)"},
+    {"clip", (PyCFunction)(void*)py_clip, METH_FASTCALL, "(grads, max_norm, out)"},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "g1nn_torch", "The policy operators on torch tensors", -1, kMethods,
+                       nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_g1nn_torch() { return PyModule_Create(&kModule); }
