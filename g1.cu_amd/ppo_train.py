@@ -3,6 +3,7 @@ g1_rollout (all N worlds for H control steps on the GPU, trajectories written in
 buffers in place), then GAE and clipped-PPO epochs in torch on the same buffers.
 
     python g1.cu_amd/ppo_train.py [--iters 600] [--worlds 8192] [--horizon 32] [--csv out.csv]
+    python g1.cu_amd/ppo_train.py --policy gated [--width 256 --hidden 512 --depth 2] [--act-q8]
 
 The trajectory contract is the reference driver's (scripts/ppo_fused.py:35-44,82-106). The
 weights are packed in the ABI's order (hidden layers W, b; mu head W, b; value head W, b;
@@ -11,6 +12,10 @@ the kernel used, and the running statistics are then updated from those raw obse
 Evaluation uses the host-step path (g1_env_reset / g1_env_step) with deterministic mean actions.
 The PPO settings are the reference's, so the reward curves are comparable
 (models/ppo_ckpt/reward_curve_fused.csv).
+
+--policy gated trains a residual policy of normed, gated blocks on g1nn's operators instead of the MLP. The
+one-launch rollout runs MLPs only, so this policy's rollouts go through g1_env_step, one control step a time; with
+--act-q8 the evaluations act through the blocks in 8 bits.
 """
 import argparse
 import csv
@@ -26,6 +31,7 @@ import torch.nn as nn
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import g1env  # noqa: E402
+import g1nn  # noqa: E402
 
 OBS, ACT = g1env.OBS_DIM, g1env.ACT_DIM
 
@@ -69,6 +75,66 @@ class GaussianPolicy(nn.Module):
             flat += [lin.weight.detach().flatten(), lin.bias.detach()]
         flat.append(self.log_std.detach())
         return torch.cat(flat).contiguous()
+
+
+class GatedBlock(nn.Module):
+    """The parameters of one block: down(act(gate(n)) * up(n)) of the normed stream n."""
+
+    def __init__(self, width, hidden):
+        super().__init__()
+        self.norm = nn.Parameter(torch.ones(width))
+        self.gate, self.up = nn.Linear(width, hidden), nn.Linear(width, hidden)
+        self.down = nn.Linear(hidden, width)
+
+    def forward(self, n):
+        return self.down(g1nn.gated_linear(n, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias))
+
+
+class GatedPolicy(nn.Module):
+    """Diagonal Gaussian actor with a value head on a residual trunk: each block reads the root-mean-square normed
+    stream and adds its output to it. Norms, gated projections and their gradients are g1nn's."""
+
+    def __init__(self, width=256, hidden=512, depth=2, log_std_init=-0.5):
+        super().__init__()
+        self.inp = nn.Linear(OBS, width)
+        self.blocks = nn.ModuleList(GatedBlock(width, hidden) for _ in range(depth))
+        self.norm = nn.Parameter(torch.ones(width))
+        self.mu_head = nn.Linear(width, ACT)
+        self.v_head = nn.Linear(width, 1)
+        self.log_std = nn.Parameter(torch.full((ACT,), float(log_std_init)))
+
+    def forward(self, z):
+        stream, add = self.inp(z), None
+        for b in self.blocks:
+            if add is None:
+                n = g1nn.rms_norm(stream, b.norm)
+            else:
+                n, stream = g1nn.rms_norm(add, b.norm, residual=stream)
+            add = b(n)
+        n, _ = g1nn.rms_norm(add, self.norm, residual=stream)
+        return self.mu_head(n), self.log_std, self.v_head(n).squeeze(-1)
+
+
+class ActingPolicy:
+    """A GatedPolicy's weights as they are now, for acting: the gated projections in 8 bits, on rows that the norm
+    writes in 8 bits. Called like the policy; without gradients."""
+
+    def __init__(self, policy):
+        self.policy, self.log_std = policy, policy.log_std
+        self.q8 = [g1nn.quantize_rows(b.gate.weight) + g1nn.quantize_rows(b.up.weight) for b in policy.blocks]
+
+    @torch.no_grad()
+    def __call__(self, z):
+        p = self.policy
+        stream, add = p.inp(z), None
+        for b, w in zip(p.blocks, self.q8):
+            if add is None:
+                q, scale = g1nn.rms_norm_q8(stream, b.norm)
+            else:
+                q, scale, stream = g1nn.rms_norm_q8(add, b.norm, residual=stream)
+            add = b.down(g1nn.gated_linear_q8(q, scale, *w, b.gate.bias.detach(), b.up.bias.detach()))
+        n, _ = g1nn.rms_norm(add, p.norm, residual=stream)
+        return p.mu_head(n), p.log_std, p.v_head(n).squeeze(-1)
 
 
 class ObsStats:
@@ -115,6 +181,29 @@ def collect(env, policy, stats, traj, act_noise=None, reset_noise=None):
     return nobs
 
 
+@torch.no_grad()
+def collect_steps(env, policy, stats, traj, obs):
+    """collect() for a policy that g1_rollout does not run: every control step through g1_env_step, from the raw
+    observations obs [N, 100] on the GPU. Returns the normalised observations and the raw ones after the last step."""
+    mean, var = stats.frozen()
+    device = obs.device
+    for t in range(traj.H):
+        traj.O[t] = obs
+        mu, log_std, v = policy(normalize(obs, mean, var))
+        noise = torch.randn_like(mu)
+        traj.A[t] = mu + log_std.exp() * noise
+        traj.LP[t] = (-0.5 * noise * noise - log_std - 0.5 * math.log(2 * math.pi)).sum(-1)
+        traj.V[t] = v
+        o, r, d = env.step(traj.A[t].cpu().numpy())
+        obs = torch.from_numpy(o).to(device)
+        traj.R[t] = torch.from_numpy(r).to(device)
+        traj.D[t] = torch.from_numpy(d).to(device)
+    traj.Vlast[:] = policy(normalize(obs, mean, var))[2]
+    nobs = normalize(traj.O, mean, var)
+    stats.update(traj.O.reshape(-1, OBS))
+    return nobs, obs
+
+
 def advantages(traj, gamma, lam):
     """Generalised advantage estimates [H, N] and value targets, backward over the horizon with
     episode boundaries from D (a done step does not bootstrap)."""
@@ -131,7 +220,7 @@ def advantages(traj, gamma, lam):
     return adv, adv + traj.V
 
 
-def ppo_update(policy, opt, nobs, traj, cfg):
+def ppo_update(policy, opt, nobs, traj, cfg, clip_grads=nn.utils.clip_grad_norm_):
     """Clipped-surrogate PPO epochs over the rollout's samples. Returns the last minibatch loss."""
     adv, ret = advantages(traj, cfg.gamma, cfg.lam)
     obs = nobs.reshape(-1, OBS)
@@ -156,7 +245,7 @@ def ppo_update(policy, opt, nobs, traj, cfg):
             loss = -surr.mean() + cfg.value_coef * (v - ret[idx]).pow(2).mean() - cfg.entropy_coef * entropy
             opt.zero_grad(set_to_none=True)
             loss.backward()
-            nn.utils.clip_grad_norm_(policy.parameters(), cfg.max_grad_norm)
+            clip_grads(policy.parameters(), cfg.max_grad_norm)
             opt.step()
     return float(loss.detach()), float(ret.mean())
 
@@ -190,25 +279,34 @@ def evaluate(env, policy, stats, steps=400, dt_ctrl=0.02):
                 alive_steps=float(alive.mean()), vx_mean=float((fwd / np.maximum(alive, 1) / dt_ctrl).mean()))
 
 
-def train(iters, worlds, horizon, seed=1, eval_every=25, eval_steps=400, csv_path=None, log=print):
+def train(iters, worlds, horizon, seed=1, eval_every=25, eval_steps=400, csv_path=None, log=print, gated=None,
+          act_q8=False):
+    """gated: None for the MLP on the fused rollout, or a GatedPolicy's (width, hidden, depth)."""
     torch.manual_seed(seed)
     cfg = PPOSettings()
     rows = []
     with g1env.Env(worlds, substeps=10, pgs_iters=8, seed=seed) as env:
-        policy = GaussianPolicy().cuda()
+        policy = (GaussianPolicy() if gated is None else GatedPolicy(*gated)).cuda()
         stats = ObsStats(OBS, "cuda")
         opt = torch.optim.Adam(policy.parameters(), lr=cfg.lr)
         traj = g1env.Trajectory(horizon, worlds)
-        env.reset()
+        obs = torch.from_numpy(env.reset()).cuda()
         t0 = time.time()
         for it in range(iters):
-            nobs = collect(env, policy, stats, traj)
+            if gated is None:
+                nobs = collect(env, policy, stats, traj)
+            else:
+                nobs, obs = collect_steps(env, policy, stats, traj, obs)
             rew_step = float(traj.R.mean())
-            loss, ret = ppo_update(policy, opt, nobs, traj, cfg)
+            loss, ret = ppo_update(policy, opt, nobs, traj, cfg,
+                                   nn.utils.clip_grad_norm_ if gated is None else g1nn.clip_grad_norm_)
             row = dict(iter=it, reward_per_step=rew_step, ret=ret, loss=loss,
                        steps_per_s=(it + 1) * horizon * worlds / (time.time() - t0))
             if it % eval_every == 0 or it == iters - 1:
-                row.update(evaluate(env, policy, stats, steps=eval_steps))
+                acting = ActingPolicy(policy) if gated is not None and act_q8 else policy
+                row.update(evaluate(env, acting, stats, steps=eval_steps))
+                if gated is not None:
+                    obs = torch.from_numpy(env.reset()).cuda()   # the evaluation moved the worlds
             rows.append(row)
             log(" ".join(f"{k}={v:.4g}" if isinstance(v, float) else f"{k}={v}" for k, v in row.items()))
             if csv_path:
@@ -233,11 +331,17 @@ def main():
     ap.add_argument("--eval-every", type=int, default=25)
     ap.add_argument("--eval-steps", type=int, default=400)
     ap.add_argument("--csv", default=None)
+    ap.add_argument("--policy", choices=("mlp", "gated"), default="mlp")
+    ap.add_argument("--width", type=int, default=256, help="of a gated policy's stream")
+    ap.add_argument("--hidden", type=int, default=512, help="of its blocks")
+    ap.add_argument("--depth", type=int, default=2, help="blocks")
+    ap.add_argument("--act-q8", action="store_true", help="evaluate a gated policy in 8 bits")
     a = ap.parse_args()
     if not torch.cuda.is_available():
         sys.exit("ppo_train.py needs a GPU")
     train(a.iters, a.worlds, a.horizon, a.seed, a.eval_every, a.eval_steps, a.csv,
-          log=lambda s: print(s, flush=True))
+          log=lambda s: print(s, flush=True), gated=(a.width, a.hidden, a.depth) if a.policy == "gated" else None,
+          act_q8=a.act_q8)
 
 
 if __name__ == "__main__":

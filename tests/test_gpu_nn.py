@@ -603,3 +603,53 @@ def test_graph_capture(nn):
         eager = {k: v if k == "out" else v.detach().clone().requires_grad_(v.requires_grad) for k, v in t.items()}
         eager["out"] = [torch.empty_like(o) for o in t["out"]]
         assert all(torch.equal(a, b) for a, b in zip(got, _everything(nn, eager))), seed
+
+
+def test_twice_differentiated_is_refused(nn):
+    """A graph of the gradients is refused, not answered with zeros."""
+    torch = _torch()
+    x, w = torch.randn(3, 8, device="cuda", requires_grad=True), torch.ones(8, device="cuda")
+    for y in (nn.rms_norm(x, w), nn.gated_linear(x, torch.randn(4, 8, device="cuda"), torch.randn(4, 8, device="cuda"))):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_clipping_in_place_is_seen_by_autograd(nn):
+    """A tensor that a graph has saved is not silently changed under it."""
+    torch = _torch()
+    a, g = torch.ones(4, device="cuda", requires_grad=True), torch.full((4,), 5.0, device="cuda")
+    y = (a * g).sum()
+    nn.clip_grad_norm([g], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_refusals_on_the_gpu(nn):
+    """Types, shapes, layouts and places that the kernels do not take."""
+    torch = _torch()
+    x, w = torch.randn(4, 8, device="cuda"), torch.ones(8, device="cuda")
+    wg = torch.randn(6, 8, device="cuda")
+    q, s = nn.rms_norm_q8(x, w)
+    qg, sg = nn.quantize_rows(wg)
+    bad = [
+        lambda: nn.rms_norm(x.double(), w.double()), lambda: nn.rms_norm(x, w.bfloat16()), lambda: nn.rms_norm(x, w[:7]),
+        lambda: nn.rms_norm(x, w.cpu()), lambda: nn.rms_norm(x, None), lambda: nn.rms_norm(x, w, residual=x[:2]),
+        lambda: nn.rms_norm(x, w, residual=x.bfloat16()), lambda: nn.rms_norm(x.t(), torch.ones(4, device="cuda")),
+        lambda: nn.rms_norm(torch.zeros(1, 32769, device="cuda"), torch.ones(32769, device="cuda")),
+        lambda: nn.rms_norm(torch.zeros(2, 0, device="cuda"), torch.ones(0, device="cuda")),
+        lambda: nn.rms_norm(x[:, ::2], torch.ones(4, device="cuda")),
+        lambda: nn.gated_linear(x, wg, wg[:5]), lambda: nn.gated_linear(x, wg[:, :7], wg[:, :7]),
+        lambda: nn.gated_linear(x, wg, wg, torch.ones(5, device="cuda")), lambda: nn.gated_linear(x, wg, wg, activation="relu"),
+        lambda: nn.gated_linear(x, wg.t(), wg.t()), lambda: nn.gated_linear(x, wg, wg.bfloat16()),
+        lambda: nn.gated_linear_q8(x, s, qg, sg, qg, sg), lambda: nn.gated_linear_q8(q, s[:3], qg, sg, qg, sg),
+        lambda: nn.gated_linear_q8(q, s, qg, sg, qg[:5], sg), lambda: nn.gated_linear_q8(q, s, qg, sg.double(), qg, sg),
+        lambda: nn.gated_linear_q8(q, s, qg, None, qg, sg), lambda: nn.gated_linear_q8(q, s, qg, sg, qg, sg, dtype=torch.half),
+        lambda: nn.clip_grad_norm([x, x.cpu()], 1.0), lambda: nn.clip_grad_norm([x.half()], 1.0),
+        lambda: nn.clip_grad_norm([x.t()], 1.0), lambda: nn.clip_grad_norm([x], 1.0, out=[]),
+        lambda: nn.clip_grad_norm([x], 1.0, out=[x[:2]]), lambda: nn.clip_grad_norm([x], -1.0),
+        lambda: nn.clip_grad_norm([x], float("nan")), lambda: nn.clip_grad_norm([x], 1.0, out=[x.cpu()]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(i)
