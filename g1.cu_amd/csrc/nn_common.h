@@ -16,24 +16,25 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T, int VEC>
 struct Elems {
   typedef T V __attribute__((ext_vector_type(VEC)));
-  static __device__ __forceinline__ T part(V v, int i) { return v[i]; }
   static __device__ __forceinline__ void load(const T* p, float (&o)[VEC]) {
     const V v = *reinterpret_cast<const V*>(p);
 #pragma unroll
     for (int i = 0; i < VEC; i++) o[i] = (float)v[i];
   }
+  // PAST: past the caches, for outputs that are larger than what they hold
+  template <bool PAST = false>
   static __device__ __forceinline__ void store(T* p, const float (&o)[VEC]) {
     V v;
 #pragma unroll
     for (int i = 0; i < VEC; i++) v[i] = (T)o[i];
-    *reinterpret_cast<V*>(p) = v;
+    if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+    else *reinterpret_cast<V*>(p) = v;
   }
 };
 template <typename T>
 struct Elems<T, 1> {
-  typedef T V;
-  static __device__ __forceinline__ T part(V v, int) { return v; }
   static __device__ __forceinline__ void load(const T* p, float (&o)[1]) { o[0] = (float)*p; }
+  template <bool PAST = false>
   static __device__ __forceinline__ void store(T* p, const float (&o)[1]) { *p = (T)o[0]; }
 };
 

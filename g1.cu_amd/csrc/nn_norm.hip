@@ -6,13 +6,45 @@
 //   8 bits: u = h w, a = max|u|, q = rint(u 127/a), scale = (a / 127) s
 //
 // All of them move each value once and are bound by memory: a row stays in the registers of the TPR threads that share
-// it (16 lanes to a whole block, by the row's length) between the reduction and the store.
+// it (16 lanes to a whole block, by the row's length) between the reduction and the store, 16 bytes an access. Rows may
+// begin at any element: the accesses need no more than its alignment (the GPU splits what crosses a line), and the last
+// one of a row that 16 bytes do not divide goes element by element.
 #include "../../include/g1nn.h"
 #include "nn_common.h"
 
 namespace g1nn {
 
 constexpr int kMaxRow = 32768;
+
+template <typename T>
+constexpr int kVec = 16 / sizeof(T);
+
+// kVec elements at p, of which `left` belong to the row; the others are zeros. EVEN: the row's length is a multiple of kVec.
+template <typename T, bool EVEN>
+struct Row {
+  static constexpr int VEC = kVec<T>;
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  typedef T Any __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  static __device__ __forceinline__ V load(const T* p, int left) {
+    if (EVEN || left >= VEC) return *reinterpret_cast<const Any*>(p);
+    V v;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = j < left ? p[j] : (T)0.0f;
+    return v;
+  }
+  static __device__ __forceinline__ void store(T* p, int left, const float (&o)[VEC]) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = (T)o[j];
+    if (EVEN || left >= VEC) {
+      *reinterpret_cast<Any*>(p) = v;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; j++)
+      if (j < left) p[j] = v[j];
+  }
+};
 
 struct NormArgs {
   long M;
@@ -24,9 +56,9 @@ struct NormArgs {
   float* rstd;   // the 8-bit form: the scales
 };
 
-template <typename T, int VEC, int TPR, int NV, bool Q8>
+template <typename T, bool EVEN, int TPR, int NV, bool Q8>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) {
-  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
+  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR, VEC = kVec<T>;
   __shared__ float part[32];
   __shared__ unsigned most[32];
   const int lane = threadIdx.x % TPR;
@@ -34,7 +66,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) 
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int k = (i * TPR + lane) * VEC;
-    if (k < a.K) Elems<T, VEC>::load((const T*)a.w + k, w[i]);
+    if (k < a.K) {
+      const auto v = Row<T, EVEN>::load((const T*)a.w + k, a.K - k);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) w[i][j] = (float)v[j];
+    }
   }
   int turn = 0;
   // every thread of a block makes the same number of turns where the block shares a row (kRows = 1)
@@ -47,13 +83,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) 
     for (int i = 0; i < NV; i++) {
       const int k = (i * TPR + lane) * VEC;
       if (k < a.K) {
-        Elems<T, VEC>::load(x + k, h[i]);
-        if (r) {
-          float e[VEC];
-          Elems<T, VEC>::load(r + k, e);
+        const auto v = Row<T, EVEN>::load(x + k, a.K - k);
 #pragma unroll
-          for (int j = 0; j < VEC; j++) h[i][j] += e[j];
-          Elems<T, VEC>::store((T*)a.h + row * a.K + k, h[i]);
+        for (int j = 0; j < VEC; j++) h[i][j] = (float)v[j];
+        if (r) {
+          const auto e = Row<T, EVEN>::load(r + k, a.K - k);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) h[i][j] += (float)e[j];
+          Row<T, EVEN>::store((T*)a.h + row * a.K + k, a.K - k, h[i]);
         }
 #pragma unroll
         for (int j = 0; j < VEC; j++) sq = __builtin_fmaf(h[i][j], h[i][j], sq);
@@ -69,7 +106,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) 
         if (k < a.K) {
 #pragma unroll
           for (int j = 0; j < VEC; j++) h[i][j] = h[i][j] * s * w[i][j];
-          Elems<T, VEC>::store((T*)a.y + row * a.K + k, h[i]);
+          Row<T, EVEN>::store((T*)a.y + row * a.K + k, a.K - k, h[i]);
         }
       }
     } else {
@@ -113,13 +150,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm(NormArgs a) 
       for (int i = 0; i < NV; i++) {
         const int k = (i * TPR + lane) * VEC;
         if (k < a.K) {
-          typedef signed char B __attribute__((ext_vector_type(VEC == 1 ? 2 : VEC)));
+          typedef signed char B __attribute__((ext_vector_type(VEC), aligned(1)));
           B b;
 #pragma unroll
           for (int j = 0; j < VEC; j++) b[j] = inv == 0 ? 0 : (signed char)(int)rintf(h[i][j] * inv);
           signed char* q = (signed char*)a.y + row * a.K + k;
-          if (VEC == 1) *q = b[0];
-          else *reinterpret_cast<B*>(q) = b;
+          if (EVEN || a.K - k >= VEC) {
+            *reinterpret_cast<B*>(q) = b;
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+              if (j < a.K - k) q[j] = b[j];
+          }
         }
       }
     }
@@ -136,9 +178,9 @@ struct NormGradArgs {
   float* dw;   // [gridDim.x][K] sums of a block's rows, or null
 };
 
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, bool EVEN, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGradArgs a) {
-  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
+  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR, VEC = kVec<T>;
   __shared__ float part[32];
   __shared__ float cols[kRows > 1 ? kBlock * VEC * NV : 1];
   const int lane = threadIdx.x % TPR;
@@ -146,14 +188,17 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int k = (i * TPR + lane) * VEC;
-    if (k < a.K) Elems<T, VEC>::load((const T*)a.w + k, w[i]);
+    if (k < a.K) {
+      const auto v = Row<T, EVEN>::load((const T*)a.w + k, a.K - k);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) w[i][j] = (float)v[j];
+    }
 #pragma unroll
     for (int j = 0; j < VEC; j++) dw[i][j] = 0;
   }
   // rows that leave registers for it: the next one is on its way while this one is summed, as it lies in memory
   constexpr bool kAhead = NV * VEC <= 16;
-  typedef typename Elems<T, VEC>::V V;
-  V dyv[NV], hv[NV], dhv[NV];
+  typename Row<T, EVEN>::V dyv[NV], hv[NV], dhv[NV];
   float s = 0;
   const long step = (long)gridDim.x * kRows;
   auto fetch = [&](long row) {
@@ -162,9 +207,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
     for (int i = 0; i < NV; i++) {
       const int k = (i * TPR + lane) * VEC;
       if (k < a.K) {
-        dyv[i] = *reinterpret_cast<const V*>((const T*)a.dy + row * a.dys + k);
-        hv[i] = *reinterpret_cast<const V*>((const T*)a.h + row * a.hs + k);
-        if (a.dh) dhv[i] = *reinterpret_cast<const V*>((const T*)a.dh + row * a.dhs + k);
+        dyv[i] = Row<T, EVEN>::load((const T*)a.dy + row * a.dys + k, a.K - k);
+        hv[i] = Row<T, EVEN>::load((const T*)a.h + row * a.hs + k, a.K - k);
+        if (a.dh) dhv[i] = Row<T, EVEN>::load((const T*)a.dh + row * a.dhs + k, a.K - k);
       }
     }
   };
@@ -182,9 +227,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
       if (k < a.K) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
-          const float dy = (float)Elems<T, VEC>::part(dyv[i], j);
-          h[i][j] = (float)Elems<T, VEC>::part(hv[i], j) * now;
-          e[i][j] = a.dh ? (float)Elems<T, VEC>::part(dhv[i], j) : 0.0f;
+          const float dy = (float)dyv[i][j];
+          h[i][j] = (float)hv[i][j] * now;
+          e[i][j] = a.dh ? (float)dhv[i][j] : 0.0f;
           dw[i][j] = __builtin_fmaf(dy, h[i][j], dw[i][j]);
           g[i][j] = dy * w[i][j];
           c = __builtin_fmaf(g[i][j], h[i][j], c);
@@ -199,7 +244,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
       if (k < a.K) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) g[i][j] = now * __builtin_fmaf(-h[i][j], c, g[i][j]) + e[i][j];
-        Elems<T, VEC>::store((T*)a.dx + row * a.K + k, g[i]);
+        Row<T, EVEN>::store((T*)a.dx + row * a.K + k, a.K - k, g[i]);
       }
     }
   }
@@ -221,9 +266,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_norm_grad(NormGra
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int k = (i * TPR + lane) * VEC;
-    if (k < a.K)
 #pragma unroll
-      for (int j = 0; j < VEC; j++) a.dw[(long)blockIdx.x * a.K + k + j] = dw[i][j];
+    for (int j = 0; j < VEC; j++)
+      if (EVEN ? k < a.K : k + j < a.K) a.dw[(long)blockIdx.x * a.K + k + j] = dw[i][j];
   }
 }
 
@@ -246,27 +291,26 @@ __global__ __launch_bounds__(1024) void k_column_join(const float* part, int P, 
   }
 }
 
-// The forms (threads per row, accesses per thread): the fewest threads whose registers hold the row in a few accesses
-// each. VEC = 1 takes rows that 16-byte accesses do not fit (odd lengths, strides or addresses).
-template <typename T, int VEC, typename F>
+// The forms (threads per row, accesses per thread): the fewest threads whose registers hold the row in a few accesses each.
+template <typename T, bool EVEN, typename F>
 int by_row(int K, F f) {
-  const int n = (K + VEC - 1) / VEC;
-  if (n <= 16) return f.template go<T, VEC, 16, 1>();
-  if (n <= 64) return f.template go<T, VEC, 64, 1>();
-  if (n <= 128) return f.template go<T, VEC, 64, 2>();
-  if (n <= 256) return f.template go<T, VEC, 256, 1>();
-  if (n <= 512) return f.template go<T, VEC, 256, 2>();
-  if (n <= 1024) return f.template go<T, VEC, 256, 4>();
-  if (n <= 2048) return f.template go<T, VEC, 256, 8>();
-  if (n <= 8192) return f.template go<T, VEC, 1024, 8>();
-  if (VEC == 1) return f.template go<T, 1, 1024, 32>();
+  const int n = (K + kVec<T> - 1) / kVec<T>;
+  if (n <= 16) return f.template go<T, EVEN, 16, 1>();
+  if (n <= 64) return f.template go<T, EVEN, 64, 1>();
+  if (n <= 128) return f.template go<T, EVEN, 64, 2>();
+  if (n <= 256) return f.template go<T, EVEN, 256, 1>();
+  if (n <= 512) return f.template go<T, EVEN, 256, 2>();
+  if (n <= 1024) return f.template go<T, EVEN, 256, 4>();
+  if (n <= 2048) return f.template go<T, EVEN, 1024, 2>();
+  if (n <= 4096) return f.template go<T, EVEN, 1024, 4>();
+  if constexpr (sizeof(T) == 4) return f.template go<T, EVEN, 1024, 8>();
   return -1;
 }
 
 template <typename F>
-int by_type(int type, bool wide, int K, F f) {
-  if (type == 0) return wide ? by_row<float, 4>(K, f) : by_row<float, 1>(K, f);
-  return wide ? by_row<bf16, 8>(K, f) : by_row<bf16, 1>(K, f);
+int by_type(int type, int K, F f) {
+  if (type == 0) return K % kVec<float> == 0 ? by_row<float, true>(K, f) : by_row<float, false>(K, f);
+  return K % kVec<bf16> == 0 ? by_row<bf16, true>(K, f) : by_row<bf16, false>(K, f);
 }
 
 constexpr long kGrid = 2048;       // blocks of a forward launch: eight to a CU
@@ -281,10 +325,10 @@ template <bool Q8>
 struct Forward {
   const NormArgs& a;
   hipStream_t st;
-  template <typename T, int VEC, int TPR, int NV>
+  template <typename T, bool EVEN, int TPR, int NV>
   int go() {
     constexpr int kBlock = TPR > 256 ? TPR : 256;
-    return launch(k_rms_norm<T, VEC, TPR, NV, Q8>, dim3(grid_for(a.M, kBlock / TPR, kGrid)), dim3(kBlock), st, a);
+    return launch(k_rms_norm<T, EVEN, TPR, NV, Q8>, dim3(grid_for(a.M, kBlock / TPR, kGrid)), dim3(kBlock), st, a);
   }
 };
 
@@ -292,11 +336,11 @@ struct Backward {
   const NormGradArgs& a;
   hipStream_t st;
   long* grid;
-  template <typename T, int VEC, int TPR, int NV>
+  template <typename T, bool EVEN, int TPR, int NV>
   int go() {
     constexpr int kBlock = TPR > 256 ? TPR : 256;
     *grid = grid_for(a.M, kBlock / TPR, kGradGrid);
-    return launch(k_rms_norm_grad<T, VEC, TPR, NV>, dim3(*grid), dim3(kBlock), st, a);
+    return launch(k_rms_norm_grad<T, EVEN, TPR, NV>, dim3(*grid), dim3(kBlock), st, a);
   }
 };
 
@@ -305,11 +349,6 @@ inline bool bad_shape(int type, long M, int K) {
   if (M < 0) return refuse("a negative number of rows");
   if (K < 1 || K > kMaxRow) return refuse("rows of 1 to 32768 values are supported");
   return false;
-}
-
-inline bool fits(int type, int K, const void* p, long stride) {
-  const int vec = type == 0 ? 4 : 8;
-  return !p || (aligned(p, 16) && stride % vec == 0);
 }
 
 inline bool bad_rows(const void* p, int type) {
@@ -326,10 +365,7 @@ int forward(int type, long M, int K, const void* x, long xs, const void* r, long
   if (bad_rows(x, type) || bad_rows(r, type) || bad_rows(w, type) || bad_rows(h, type) || (!Q8 && bad_rows(y, type)))
     return -1;
   const NormArgs a{M, K, x, r, w, xs, rs, eps, y, h, rstd};
-  const int vec = type == 0 ? 4 : 8;
-  const bool wide = K % vec == 0 && fits(type, K, x, xs) && fits(type, K, r, rs) && fits(type, K, w, K) &&
-                    fits(type, K, h, K) && (Q8 ? aligned(y, vec) : fits(type, K, y, K));
-  return by_type(type, wide, K, Forward<Q8>{a, st});
+  return by_type(type, K, Forward<Q8>{a, st});
 }
 
 }  // namespace g1nn
@@ -363,9 +399,7 @@ extern "C" int g1_nn_rms_norm_backward(int type, long M, int K, const void* dy, 
         bad_rows(dw, type))
       return -1;
     const NormGradArgs a{M, K, dy, dh, h, w, dys, dhs, hs, rstd, dx, dw ? (float*)ws : nullptr};
-    const bool wide = K % (type == 0 ? 4 : 8) == 0 && fits(type, K, dy, dys) && fits(type, K, dh, dhs) &&
-                      fits(type, K, h, hs) && fits(type, K, w, K) && fits(type, K, dx, K);
-    const int rc = by_type(type, wide, K, Backward{a, st, &grid});
+    const int rc = by_type(type, K, Backward{a, st, &grid});
     if (rc) return rc;
   }
   if (!dw) return 0;
