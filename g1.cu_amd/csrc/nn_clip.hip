@@ -27,14 +27,12 @@ struct ClipTable {
   unsigned char in_type[kTable], out_type[kTable];
 };
 
+// The tensor that a chunk belongs to: the last one that begins at or before it. A lane looks at a tensor, so the search
+// is one load.
+static_assert(kTable == 64, "a lane to a tensor");
 __device__ __forceinline__ int tensor_of(const ClipTable& t, int chunk) {
-  int lo = 0, hi = t.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.first[mid] <= chunk) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < t.n && t.first[lane] <= chunk)) - 1);
 }
 
 __device__ __forceinline__ double block_sum(double v, double* part) {

@@ -136,8 +136,8 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
         const int row = c_row<S>(i, r);
         float g, u;
         if constexpr (sizeof(T) == 1) {
-          g = (float)acc[i][j][r] * (given[r] * sg) + bg;
-          u = (float)acc[i][j + 1][r] * (given[r] * su) + bu;
+          g = __builtin_fmaf((float)acc[i][j][r], given[r] * sg, bg);
+          u = __builtin_fmaf((float)acc[i][j + 1][r], given[r] * su, bu);
         } else {
           g = acc[i][j][r] + bg;
           u = acc[i][j + 1][r] + bu;
@@ -406,8 +406,8 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
     float gate, up;
     if constexpr (sizeof(T) == 1) {
       const float s = a.s[lane];
-      gate = (float)gm * (s * a.sg[f]) + (a.bg ? ((const float*)a.bg)[f] : 0);
-      up = (float)um * (s * a.su[f]) + (a.bu ? ((const float*)a.bu)[f] : 0);
+      gate = __builtin_fmaf((float)gm, s * a.sg[f], a.bg ? ((const float*)a.bg)[f] : 0);
+      up = __builtin_fmaf((float)um, s * a.su[f], a.bu ? ((const float*)a.bu)[f] : 0);
     } else {
       gate = gm + (in && a.bg ? (float)((const T*)a.bg)[f] : 0);
       up = um + (in && a.bu ? (float)((const T*)a.bu)[f] : 0);

@@ -653,3 +653,50 @@ def test_refusals_on_the_gpu(nn):
         with pytest.raises(ValueError):
             call()
             raise AssertionError(i)
+
+
+# ------------------------------------------------------------------------------------ large tiles
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "q8"])
+@pytest.mark.parametrize("M,K,F", [(4200, 72, 1032), (8200, 40, 2056), (16500, 512, 24), (4100, 1030, 520)])
+def test_gated_in_large_tiles(nn, M, K, F, dtype):
+    """Products with enough tiles for the large and the huge ones (128 x 128 from 256 on, 256 x 128 from 1024 on, for the
+    gradients' products too), their edges and lengths odd. The 64-bit values are computed on the GPU."""
+    torch = _torch()
+    if dtype == "q8":
+        rng = np.random.default_rng(K)
+        q, qg, qu = (torch.from_numpy(rng.integers(-127, 128, s).astype(np.int8)).cuda() for s in ((M, K), (F, K), (F, K)))
+        s, sg = torch.rand(M, device="cuda") / 127, torch.rand(F, device="cuda") / (127 * math.sqrt(K))
+        g = (q.double() @ qg.double().t().contiguous()) * s.double()[:, None] * sg.double()
+        u = (q.double() @ qu.double().t().contiguous()) * s.double()[:, None] * sg.double()
+        a, _ = _act_ref(g, "silu")
+        ea = 1.2 * 8 * U * g.abs() + 16 * U * (1 + g.abs() + g.abs() ** 3)
+        bound = ea * u.abs() + a.abs() * 8 * U * u.abs() + 4 * U * (a * u).abs()
+        for dt, o in ((torch.float32, 0), (torch.bfloat16, 2.0 ** -8)):
+            y = nn.gated_linear_q8(q, s, qg, sg, qu, sg, dtype=dt)
+            assert bool(((y.double() - a * u).abs() <= bound + o * (a * u).abs()).all()), dt
+        return
+    ins = [t.cuda() for t in _gated_inputs(M, K, F, dtype, K + F)]
+    ref = _GatedRef(*ins[:5], "silu", ins[5], dtype)
+    dev = [t.requires_grad_() for t in ins[:5]]
+    y = nn.gated_linear(*dev)
+    got = [y, *torch.autograd.grad(y, dev, ins[5])]
+    for v, (r, b), name in zip(got, [(ref.y, ref.by), *ref.grads], ("y", "dx", "dwg", "dwu", "dbg", "dbu")):
+        far = (v.detach().double() - r).abs() - b
+        assert bool((far <= 0).all()), (name, float(far.max()))
+
+
+def test_gated_values_without_size_in_large_tiles(nn):
+    torch = _torch()
+    x, wg, wu, bg, bu, _ = _cuda(_gated_inputs(4200, 72, 1032, "fp32", 5))
+    plain = nn.gated_linear(x, wg, wu, bg, bu, activation="sigmoid")
+    z = x.clone()
+    z[130, 70], z[4199, 0] = float("inf"), float("nan")
+    g, u = z[[130, 4199]].double() @ wg.double().t().contiguous() + bg, z[[130, 4199]].double() @ wu.double().t().contiguous() + bu
+    ref = _act_ref(g, "sigmoid")[0] * u
+    got = nn.gated_linear(z, wg, wu, bg, bu, activation="sigmoid")
+    rest = torch.ones(4200, dtype=torch.bool, device="cuda")
+    rest[[130, 4199]] = False
+    assert torch.equal(got[rest], plain[rest])
+    assert torch.equal(torch.isnan(got[[130, 4199]]), torch.isnan(ref))
+    m = torch.isinf(ref)
+    assert bool(m.any()) and torch.equal(got[[130, 4199]][m].double(), ref[m])
