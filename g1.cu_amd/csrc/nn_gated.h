@@ -6,8 +6,15 @@
 //
 // Forward: one product whose tile holds both projections of its outputs; activation and product in the epilogue.
 // Backward: the same product again with an epilogue that reads dy and writes d = [dg | du] (it costs 4 K operations a
-// value and saves writing and reading g and u), then dx = d [Wg; Wu], then [dWg; dWu] = d^T x with the rows split
-// over the blocks, and a join of those parts and of the column sums in a fixed order. d is held in the tensors' type.
+// value and saves writing and reading g and u, and the rounding of both), then dx = d [Wg; Wu], then [dWg; dWu] = d^T x
+// with the rows split over the blocks, and a join of those parts and of the column sums in a fixed order. d is held in
+// the tensors' type: for bf16 that is a rounding of each of its values to 8 bits, what the matrix cores read.
+//
+// Measured, 65536 rows: bf16 512 x 2048 forward 325 us (845 TFLOP/s), d 465 us, dx 305 us (900), dW 278 us (990), join 18 us;
+// fp32 256 x 512 forward 181 us (190 TFLOP/s of fp32 products), d 218 us, dx 205 us (167), dW 200 us (171), join 10 us. A plain
+// matrix product of these shapes by the vendor's library runs at 730 (forward), 930 (dx) and 490 (dW) TFLOP/s in bf16, 121 in
+// fp32; its best here is 1405 and 154, at 8192 cubed. Bound: the products by the operands' way through L2 and LDS
+// between two barriers (matrix units busy 40 to 45 % of the time), d also by its 805 MB of dy and d.
 #pragma once
 #include <algorithm>
 #include <initializer_list>
@@ -87,7 +94,9 @@ struct Tiles<float> {
 };
 
 // Which of them a product of m x n takes: the large ones where they give every CU a block, the huge ones (which read
-// less from the L2s: 96 instead of 128 rows for as many products) where they give every CU four.
+// less from the L2s: 96 instead of 128 rows for as many products) where they give every CU four. Measured, us, small to
+// large: fp32 256 x 512, 2048 rows 11.7 to 14.4, 4096 rows 19.6 to 17.4; bf16 512 x 1024, 1024 rows 6.9 to 8.6, 2048 rows
+// 11.6 to 9.3. Large to huge, bf16 65536 x 512 x 2048: forward 357 to 335, dx 331 to 306.
 enum Size { kSmall, kLarge, kHuge };
 inline Size size_of(long m, long n) {
   if (((m + 255) / 256) * ((n + 127) / 128) >= 1024) return kHuge;
@@ -322,8 +331,10 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, int wide, int 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
-// Up to 8 rows: a wave takes an output, reads its two rows of weights once, 16 bytes a lane, and multiplies all of
-// the rows of x with them. Bound by the weights' way from memory; matrix tiles would be mostly padding.
+// A wave takes an output and up to 8 rows of x: it reads the output's two rows of weights once, 16 bytes a lane, and
+// multiplies all of its rows of x with them. Bound by the weights' way from memory and, with more rows, by those of x from
+// L2; matrix tiles would be mostly padding, and one of them alone on a CU waits for every turn. One row of 256 into 512 fp32
+// outputs takes 2.9 us, one of 1024 into 2731 in 8 bits 3.3 us, about an empty launch.
 template <typename T>
 struct Dot {
   static constexpr int kVec = 16 / sizeof(T);
@@ -370,6 +381,7 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
   typedef typename Dot<T>::Acc Acc;
   constexpr int VEC = WIDE ? Dot<T>::kVec : 1;
   const int lane = threadIdx.x & 63, f = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int row0 = blockIdx.y * ROWS, rows = min(ROWS, a.M - row0), row = row0 + lane;   // lane m takes row m of them
   if (f >= (GRAD ? a.half : a.F)) return;
   const bool in = f < a.F;
   const T* wg = (const T*)a.wg + (in ? f : 0) * a.wgs;
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
     Dot<T>::load(wu + k, q);
 #pragma unroll
     for (int m = 0; m < ROWS; m++) {
-      Dot<T>::load((const T*)a.x + (m < a.M ? m : 0) * a.xs + k, x);
+      Dot<T>::load((const T*)a.x + (row0 + (m < rows ? m : 0)) * a.xs + k, x);
       Dot<T>::add(p, x, g[m]);
       Dot<T>::add(q, x, u[m]);
     }
@@ -394,7 +406,6 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
       g[m] += __shfl_xor(g[m], d);
       u[m] += __shfl_xor(u[m], d);
     }
-  // lane m takes row m
   Acc gm = g[0], um = u[0];
 #pragma unroll
   for (int m = 1; m < ROWS; m++) {
@@ -402,10 +413,10 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
     um = lane == m ? u[m] : um;
   }
   float dg = 0, du = 0;
-  if (lane < a.M) {
+  if (lane < rows) {
     float gate, up;
     if constexpr (sizeof(T) == 1) {
-      const float s = a.s[lane];
+      const float s = a.s[row];
       gate = __builtin_fmaf((float)gm, s * a.sg[f], a.bg ? ((const float*)a.bg)[f] : 0);
       up = __builtin_fmaf((float)um, s * a.su[f], a.bu ? ((const float*)a.bu)[f] : 0);
     } else {
@@ -420,14 +431,14 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
       default: v = activation<GRAD>(3, gate, d);
     }
     if constexpr (!GRAD) {
-      ((O*)a.y)[(long)lane * a.F + f] = (O)(v * up);
+      ((O*)a.y)[(long)row * a.F + f] = (O)(v * up);
     } else {
       if (in) {
-        const float dy = (float)((const T*)a.dy)[lane * a.dys + f];
+        const float dy = (float)((const T*)a.dy)[row * a.dys + f];
         dg = dy * up * d;
         du = dy * v;
       }
-      T* to = (T*)a.d + (long)lane * (2 * a.half) + f;   // zeros from F to `half`
+      T* to = (T*)a.d + (long)row * (2 * a.half) + f;   // zeros from F to `half`
       to[0] = (T)dg;
       to[a.half] = (T)du;
     }
@@ -440,8 +451,9 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs a) {
         du += __shfl_xor(du, d);
       }
       if (lane == 0) {
-        a.sums[f] = dg;
-        a.sums[a.half + f] = du;
+        float* at = a.sums + (long)blockIdx.y * (2 * a.half) + f;
+        at[0] = dg;
+        at[a.half] = du;
       }
     }
   }
@@ -474,20 +486,24 @@ int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
 
 template <typename T, typename O, int ROWS, bool GRAD>
 int run_few(const GatedArgs& a, bool wide, hipStream_t st) {
-  const dim3 grid(((GRAD ? a.half : a.F) + 3) / 4);
+  const dim3 grid(((GRAD ? a.half : a.F) + 3) / 4, (a.M + ROWS - 1) / ROWS);
   if (wide) return launch(k_gated_few<T, O, ROWS, true, GRAD>, grid, dim3(256), st, a);
   return launch(k_gated_few<T, O, ROWS, false, GRAD>, grid, dim3(256), st, a);
 }
 
-constexpr int kFew = 8;
+// Up to how many rows. Measured against small tiles (K x F; us a forward call): fp32, whose tiles wait longest, 8 rows of
+// 256 x 512 4.0 to 8.0 and of 1024 x 2048 8.4 to 19.8, 32 rows 4.8 to 9.3 and 17.8 to 21.2. bf16, 4 rows of 1024 x 4096 5.9
+// to 8.5, but 8 rows 9.6 to 8.8; 8 bits, 4 rows of 1024 x 2731 4.3 to 5.6, 8 rows 6.3 to 5.6.
+template <typename T>
+constexpr int kFew = sizeof(T) == 4 ? 32 : 4;
 
 template <typename T, typename O, bool GRAD>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
-  if (a.M <= kFew) {
+  if (a.M <= kFew<T>) {
     if (a.M == 1) return run_few<T, O, 1, GRAD>(a, wide, st);
     if (a.M == 2) return run_few<T, O, 2, GRAD>(a, wide, st);
     if (a.M <= 4) return run_few<T, O, 4, GRAD>(a, wide, st);
-    return run_few<T, O, 8, GRAD>(a, wide, st);
+    if constexpr (kFew<T> > 4) return run_few<T, O, 8, GRAD>(a, wide, st);
   }
   switch (a.act) {
     case 0: return run_gated<T, O, GRAD, 0>(a, wide, st);
@@ -526,8 +542,10 @@ int run_dw(const GatedArgs& a, Size s, bool wide, hipStream_t st) {
 }
 
 // How the long sums are split. [dWg; dWu] over the rows: as many parts as give two blocks to each CU, of 256 rows at
-// least, and a multiple of eight (one L2 each) from three on. dx over the outputs, only where its tiles leave CUs idle:
-// parts of 128 outputs of both projections at least.
+// least, and a multiple of eight (one L2 each) from three on: bf16 65536 x 512 x 2048 takes 310 us in 8 parts, 560 in 4
+// (half of the L2s) and 355 in 16. dx over the outputs, only where its tiles leave CUs idle: parts of 128 outputs of
+// both projections at least (fp32 us, whole to parts: 1 row 256 x 512 24.6 to 11.6, 64 rows 256 x 2048 86 to 15, 1024 rows
+// 512 x 1024 46 to 32).
 struct Split {
   int half, splits, chunk, xsplits, xchunk;
   Size w, x;
@@ -578,7 +596,7 @@ int gated_backward(GatedArgs a, const Split& s, hipStream_t st) {
   if (!biases) a.sums = nullptr;
   using Large = typename Tiles<T>::Large;
   using Small = typename Tiles<T>::Small;
-  a.sum_rows = a.M <= kFew                        ? 1
+  a.sum_rows = a.M <= kFew<T>                     ? (a.M + 7) / 8
                : gated_size<true>(a) == kLarge ? (a.M + Large::BM - 1) / Large::BM * Large::WM
                                                : (a.M + Small::BM - 1) / Small::BM * Small::WM;
   if (a.M > 0) {

@@ -9,6 +9,9 @@
 // it (16 lanes to a whole block, by the row's length) between the reduction and the store, 16 bytes an access. Rows may
 // begin at any element: the accesses need no more than its alignment (the GPU splits what crosses a line), and the last
 // one of a row that 16 bytes do not divide goes element by element.
+// Measured: 65536 x 256 fp32 with the residual 43 us forward and 43 us backward (6.2 TB/s, partly from the last-level
+// cache; a large copy moves 5.0), dw's join 4 us; 65536 x 2048 bf16 188 and 220 us (5.7 and 4.9 TB/s), join 5.6 us; 8 bits of
+// 8191 x 1999 fp32 36 us (5.9 TB/s). One row of 1024 takes 3 us, about an empty launch.
 #include "../../include/g1nn.h"
 #include "nn_common.h"
 
@@ -292,6 +295,8 @@ __global__ __launch_bounds__(1024) void k_column_join(const float* part, int P, 
 }
 
 // The forms (threads per row, accesses per thread): the fewest threads whose registers hold the row in a few accesses each.
+// From 256 accesses on a block shares a row: 256 threads of one access each took 220 us for the gradients of 65536 rows of
+// 2048 bf16 values, 64 threads of four 287 us (their registers leave fewer waves to wait for memory).
 template <typename T, bool EVEN, typename F>
 int by_row(int K, F f) {
   const int n = (K + kVec<T> - 1) / kVec<T>;
