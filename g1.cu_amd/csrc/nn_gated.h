@@ -79,7 +79,7 @@ struct GatedArgs {
 };
 
 // Tiles of a block by type, four chunks deep, and eight where a block is small and waits more; in fp32 (three planes) half
-// of that.
+// of that, and eight again in the tiny ones, which only the fp32 projections have.
 template <typename T>
 struct Tiles {
   using Huge = Shape<256, 128, 2, 2, 4>;
@@ -91,13 +91,14 @@ struct Tiles<float> {
   using Huge = Shape<128, 128, 2, 2, 2>;
   using Large = Huge;
   using Small = Shape<64, 64, 2, 1, 4, 2>;
+  using Tiny = Shape<32, 64, 1, 1, 8, 4>;
 };
 
 // Which of them a product of m x n takes: the large ones where they give every CU a block, the huge ones (which read
 // less from the L2s: 96 instead of 128 rows for as many products) where they give every CU four. Measured, us, small to
 // large: fp32 256 x 512, 2048 rows 11.7 to 14.4, 4096 rows 19.6 to 17.4; bf16 512 x 1024, 1024 rows 6.9 to 8.6, 2048 rows
 // 11.6 to 9.3. Large to huge, bf16 65536 x 512 x 2048: forward 357 to 335, dx 331 to 306.
-enum Size { kSmall, kLarge, kHuge };
+enum Size { kTiny, kSmall, kLarge, kHuge };
 inline Size size_of(long m, long n) {
   if (((m + 255) / 256) * ((n + 127) / 128) >= 1024) return kHuge;
   return ((m + 127) / 128) * ((n + 127) / 128) >= 256 ? kLarge : kSmall;
@@ -183,7 +184,7 @@ __device__ __forceinline__ void gated_out(const GatedArgs& a, int m, int f0, con
 }
 
 template <typename T, typename O, typename S, bool WIDE, bool GRAD, int ACT>
-__global__ __launch_bounds__(S::kThreads, S::KS == 2 ? 1 : sizeof(T) == 4 ? 3 : 2) void k_gated(GatedArgs a) {
+__global__ __launch_bounds__(S::kThreads, S::KS > 1 ? 1 : sizeof(T) == 4 ? 3 : 2) void k_gated(GatedArgs a) {
   G1NN_LDS(T, S, WIDE);
   const int cover = GRAD ? a.half : a.F, tm = (a.M + S::BM - 1) / S::BM, tn = (cover + S::BN / 2 - 1) / (S::BN / 2);
   int m, n;
@@ -467,20 +468,26 @@ int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
   return launch(k_gated<T, O, S, false, GRAD, ACT>, grid, dim3(S::kThreads), st, a);
 }
 
-// (the gradients' epilogue leaves no registers for a huge tile's accumulators)
-template <bool GRAD>
+// The projections' tiles. The gradients' epilogue leaves no registers for a huge tile's accumulators. In fp32, whose
+// small tiles take longest, tiny ones where no CU gets two of them (us, small to tiny: 40 rows 256 x 512 9.7 to 7.1, 1000
+// rows 256 x 256 9.7 to 7.5, 64 rows 1000 x 2000 21.3 to 17.5; bf16 gains nothing, 64 rows 1000 x 2000 7.9 to 8.5).
+template <typename T, bool GRAD>
 Size gated_size(const GatedArgs& a) {
   const Size s = size_of(a.M, 2l * a.F);
-  return GRAD && s == kHuge ? kLarge : s;
+  if (GRAD && s == kHuge) return kLarge;
+  return sizeof(T) == 4 && s == kSmall && ((a.M + 31) / 32) * ((2l * a.F + 63) / 64) <= 256 ? kTiny : s;
 }
 
 template <typename T, typename O, bool GRAD, int ACT>
 int run_gated(const GatedArgs& a, bool wide, hipStream_t st) {
-  const Size s = gated_size<GRAD>(a);
+  const Size s = gated_size<T, GRAD>(a);
   if constexpr (!GRAD) {
     if (s == kHuge) return run_gated<T, O, typename Tiles<T>::Huge, GRAD, ACT>(a, wide, st);
   }
   if (s == kLarge) return run_gated<T, O, typename Tiles<T>::Large, GRAD, ACT>(a, wide, st);
+  if constexpr (sizeof(T) == 4) {
+    if (s == kTiny) return run_gated<T, O, typename Tiles<T>::Tiny, GRAD, ACT>(a, wide, st);
+  }
   return run_gated<T, O, typename Tiles<T>::Small, GRAD, ACT>(a, wide, st);
 }
 
@@ -575,7 +582,7 @@ struct Workspace {
   Workspace(int type, long M, int K, const Split& s) {
     d = 0;
     sums = d + round16(M * 2 * s.half * (type == 0 ? 4 : 2));
-    // rows of column sums: ceil(M / BM) WM of them, two for every 128 rows with large tiles, four with small ones
+    // rows of column sums: ceil(M / BM) WM of them, two for every 128 rows with large tiles, four with smaller ones
     parts = sums + round16((M + 127) / 128 * 4 * 2 * s.half * 4);
     xparts = parts + round16((long)s.splits * 2 * s.half * K * 4);
     bytes = xparts + (s.xsplits > 1 ? s.xsplits * M * K * 4 : 0);
@@ -594,11 +601,15 @@ int gated_backward(GatedArgs a, const Split& s, hipStream_t st) {
   const bool wide = xw && even(a.wg, a.wgs, a.K, size, 16) && even(a.wu, a.wus, a.K, size, 16);
   const bool weights = a.dwg || a.dwu, biases = a.dbg || a.dbu;
   if (!biases) a.sums = nullptr;
-  using Large = typename Tiles<T>::Large;
-  using Small = typename Tiles<T>::Small;
-  a.sum_rows = a.M <= kFew<T>                     ? (a.M + 7) / 8
-               : gated_size<true>(a) == kLarge ? (a.M + Large::BM - 1) / Large::BM * Large::WM
-                                               : (a.M + Small::BM - 1) / Small::BM * Small::WM;
+  const auto rows = [&](auto shape) {
+    using S = decltype(shape);
+    return (a.M + S::BM - 1) / S::BM * S::WM;
+  };
+  const Size g = gated_size<T, true>(a);
+  a.sum_rows = a.M <= kFew<T> ? (a.M + 7) / 8 : g == kLarge ? rows(typename Tiles<T>::Large{}) : rows(typename Tiles<T>::Small{});
+  if constexpr (sizeof(T) == 4) {
+    if (a.M > kFew<T> && g == kTiny) a.sum_rows = rows(typename Tiles<T>::Tiny{});
+  }
   if (a.M > 0) {
     int rc = run_gated<T, T, true>(a, wide, st);
     if (rc) return rc;

@@ -626,3 +626,64 @@ def test_gated_values_without_size_in_large_tiles(nn):
     assert torch.equal(torch.isnan(got[[130, 4199]]), torch.isnan(ref))
     m = torch.isinf(ref)
     assert bool(m.any()) and torch.equal(got[[130, 4199]][m].double(), ref[m])
+
+
+def test_gated_gradients_past_32_bits(nn):
+    """A workspace of more than 2^31 elements: the gradients of the last rows, and of weights that only those rows move."""
+    torch = _torch()
+    M, K, F, n = 2 ** 20 + 5, 8, 1040, 5
+    tail, wg, wu, bg, bu, dtail = _cuda(_gated_inputs(n, K, F, "bf16", 8))
+    x, dy = torch.zeros(M, K, device="cuda", dtype=torch.bfloat16), torch.zeros(M, F, device="cuda", dtype=torch.bfloat16)
+    x[-n:], dy[-n:] = tail, dtail
+    ins = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    got = torch.autograd.grad(nn.gated_linear(*ins), ins, dy)
+    assert not got[0][:-n:997].any()
+    ref = _GatedRef(*[t.detach().cpu() for t in (tail, wg, wu, bg, bu)], "silu", dtail.cpu(), "bf16")
+    for v, (r, b) in zip([got[0][-n:], *got[1:]], ref.grads):
+        _within(v, r, b, "tail")
+
+
+def test_rows_of_one_and_three_dimensions(nn):
+    torch = _torch()
+    g = _gen(7)
+    x, r = (_normal(g, 2, 3, 40, dtype=torch.float32).cuda() for _ in range(2))
+    w = _normal(g, 40, dtype=torch.float32, mean=1).cuda()
+    wg, wu = (_normal(g, 24, 40, dtype=torch.float32).cuda() for _ in range(2))
+    flat = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+    y, h = nn.rms_norm(x, w, EPS, r)
+    y2, h2 = nn.rms_norm(flat(x), w, EPS, flat(r))
+    assert y.shape == x.shape and torch.equal(flat(y), y2) and torch.equal(flat(h), h2)
+    q, s, _ = nn.rms_norm_q8(x, w, EPS, r)
+    assert s.shape == (2, 3)
+    (qg, sg), (qu, su) = nn.quantize_rows(wg), nn.quantize_rows(wu)
+    z = nn.gated_linear_q8(q, s, qg, sg, qu, su)
+    assert z.shape == (2, 3, 24) and torch.equal(flat(z), nn.gated_linear_q8(flat(q), s.reshape(-1), qg, sg, qu, su))
+    ins = [t.clone().requires_grad_() for t in (x, wg, wu)]
+    z = nn.gated_linear(*ins)
+    dz = torch.randn_like(z)
+    gx, gg, gu = torch.autograd.grad(z, ins, dz)
+    flats = [t.detach().clone().requires_grad_() for t in (flat(x), wg, wu)]
+    for a, b in zip((flat(gx), gg, gu), torch.autograd.grad(nn.gated_linear(*flats), flats, flat(dz))):
+        assert torch.equal(a, b)
+    one = nn.gated_linear(x[0, 0], wg, wu)
+    assert one.shape == (24,) and torch.equal(one, nn.gated_linear(x[0, :1], wg, wu)[0])
+    q1, s1 = nn.rms_norm_q8(x[0, 0], w)
+    assert s1.shape == () and q1.shape == (40,)
+    with pytest.raises(ValueError):
+        nn.rms_norm(x.transpose(0, 1), w)
+
+
+@pytest.mark.parametrize("M,K,F", [(40, 256, 512), (100, 65, 700), (33, 30, 31), (1000, 72, 100), (9, 40, 64), (32, 128, 40),
+                                   (5, 100, 40), (17, 33, 20)])
+def test_gated_at_the_changes_of_form(nn, M, K, F):
+    """Rows on both sides of the forms' limits (a wave per output, tiny, small tiles), with gradients, whose column
+    sums are counted by form."""
+    torch = _torch()
+    for dtype in ("fp32", "bf16"):
+        ins = _gated_inputs(M, K, F, dtype, 2 * M + K)
+        ref = _GatedRef(*ins[:5], "gelu", ins[5], dtype)
+        dev = [t.cuda().requires_grad_() for t in ins[:5]]
+        y = nn.gated_linear(*dev, activation="gelu")
+        _within(y, ref.y, ref.by, (dtype, "y"))
+        for v, (r, b), name in zip(torch.autograd.grad(y, dev, ins[5].cuda()), ref.grads, ("dx", "dwg", "dwu", "dbg", "dbu")):
+            _within(v, r, b, (dtype, name))
