@@ -126,7 +126,14 @@ struct Across {
 };
 
 // ---- staging through registers: fp32, and rows that 16-byte accesses do not fit ------------------------------------
-// WIDE: the host has checked that every chunk's elements lie within the operand and can be read in aligned accesses.
+// Accesses need no more than the elements' alignment (the GPU splits what crosses a line): whole chunks are read in 16
+// bytes (8 across k) wherever they begin, and only those at the ends of k or of the columns element by element. WIDE: the
+// host has checked that there are none of the latter, and that chunks are aligned.
+template <typename V, typename T>
+__device__ __forceinline__ V read_any(const T* p) {
+  typedef V Any __attribute__((aligned(sizeof(T))));
+  return *reinterpret_cast<const Any*>(p);
+}
 template <typename T, typename Op, int ROWS, int SLOTS, int THREADS, bool WIDE, bool ALONG = Op::kAlong>
 struct Stage;
 
@@ -147,37 +154,34 @@ struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, true> {
     for (int i = 0; i < kUnits; i++) off[i] = o.offset(unit(i) / SLOTS) + unit(i) % SLOTS * kPer;
   }
   __device__ __forceinline__ void load(const Op& o, long k0) {
-    if constexpr (WIDE) {
 #pragma unroll
-      for (int i = 0; i < kUnits; i++)
+    for (int i = 0; i < kUnits; i++)
 #pragma unroll
-        for (int a = 0; a < kAcc; a++) v[i][a] = reinterpret_cast<const i32x4*>(base(o, i) + k0 + off[i])[a];
-    } else {
-      load(o, k0, k0 + SLOTS * Form<T>::kPer);
-    }
+      for (int a = 0; a < kAcc; a++) v[i][a] = read_any<i32x4>(base(o, i) + k0 + off[i] + a * (16 / sizeof(T)));
   }
   // zeros from `end`
   __device__ __forceinline__ void load(const Op& o, long k0, long end) {
+    constexpr int kIn = 4 / sizeof(T), kEach = 16 / sizeof(T);   // elements of a word, of an access
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       const T* p = base(o, i) + k0 + off[i];
       const int n = (int)(end - k0) - unit(i) % SLOTS * kPer;
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int a = 0; a < kAcc; a++) {
-          v[i][a] = i32x4{0, 0, 0, 0};
-          if (a * 16 / (int)sizeof(T) < n) v[i][a] = reinterpret_cast<const i32x4*>(p)[a];
+      for (int a = 0; a < kAcc; a++) {
+        v[i][a] = i32x4{0, 0, 0, 0};
+        // WIDE: an access that has begun is whole, or ends in zeros that are there (the padding of d)
+        if (WIDE ? a * kEach < n : (a + 1) * kEach <= n) {
+          v[i][a] = read_any<i32x4>(p + a * kEach);
+        } else if (!WIDE) {
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            unsigned word = 0;
+#pragma unroll
+            for (int e = 0; e < kIn; e++)
+              if (a * kEach + w * kIn + e < n) word |= bits(p[a * kEach + w * kIn + e]) << (e * 8 * sizeof(T));
+            v[i][a][w] = (int)word;
+          }
         }
-        continue;
-      }
-      constexpr int kIn = 4 / sizeof(T);   // elements of a word
-#pragma unroll
-      for (int w = 0; w < kPer / kIn; w++) {
-        unsigned word = 0;
-#pragma unroll
-        for (int e = 0; e < kIn; e++)
-          if (w * kIn + e < n) word |= bits(p[w * kIn + e]) << (e * 8 * sizeof(T));
-        v[i][w / 4][w % 4] = (int)word;
       }
     }
   }
@@ -219,37 +223,31 @@ struct Stage<T, Op, ROWS, SLOTS, THREADS, WIDE, false> {
       off[i] = (unsigned)(unit(i) / kWidth * 4) * (unsigned)o.stride + (unsigned)(c < o.cols ? c : 0);
     }
   }
+  // columns [0, left) of line p
+  static __device__ __forceinline__ u32x2 line(const T* p, int left) {
+    if (WIDE || left >= kCols) return read_any<u32x2>(p);
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kCols; e++)
+      if (e < left) w[e * sizeof(T) / 4] |= bits(p[e]) << (e * sizeof(T) % 4 * 8);
+    return u32x2{w[0], w[1]};
+  }
   __device__ __forceinline__ void load(const Op& o, long k0) {
-    if constexpr (WIDE) {
 #pragma unroll
-      for (int i = 0; i < kUnits; i++)
+    for (int i = 0; i < kUnits; i++)
 #pragma unroll
-        for (int l = 0; l < 4; l++) v[i][l] = *reinterpret_cast<const u32x2*>(o.p + (k0 + l) * o.stride + off[i]);
-    } else {
-      load(o, k0, k0 + SLOTS * Form<T>::kPer);
-    }
+      for (int l = 0; l < 4; l++) v[i][l] = line(o.p + (k0 + l) * o.stride + off[i], left(o, i));
   }
   __device__ __forceinline__ void load(const Op& o, long k0, long end) {
 #pragma unroll
-    for (int i = 0; i < kUnits; i++) {
-      const int left = o.cols - o.col0 - unit(i) % kWidth * kCols;
+    for (int i = 0; i < kUnits; i++)
 #pragma unroll
       for (int l = 0; l < 4; l++) {
-        const T* p = o.p + (k0 + l) * o.stride + off[i];
-        const bool ok = k0 + unit(i) / kWidth * 4 + l < end;
-        if constexpr (WIDE) {
-          v[i][l] = u32x2{0, 0};
-          if (ok) v[i][l] = *reinterpret_cast<const u32x2*>(p);
-          continue;
-        }
-        unsigned w[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < kCols; e++)
-          if (ok && e < left) w[e * sizeof(T) / 4] |= bits(p[e]) << (e * sizeof(T) % 4 * 8);
-        v[i][l] = u32x2{w[0], w[1]};
+        v[i][l] = u32x2{0, 0};
+        if (k0 + unit(i) / kWidth * 4 + l < end) v[i][l] = line(o.p + (k0 + l) * o.stride + off[i], left(o, i));
       }
-    }
   }
+  static __device__ __forceinline__ int left(const Op& o, int i) { return o.cols - o.col0 - unit(i) % kWidth * kCols; }
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
