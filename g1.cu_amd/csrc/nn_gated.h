@@ -556,11 +556,11 @@ int run_dw(const GatedArgs& a, Size s, bool wide, hipStream_t st) {
 struct Split {
   int half, splits, chunk, xsplits, xchunk;
   Size w, x;
-  Split(long M, int K, int F) {
+  Split(int type, long M, int K, int F) {   // type 0: fp32, whose huge tiles are its large ones
     half = (F + 63) / 64 * 64;
     const long most = (M + 255) / 256;
     const long huge = ((2l * half + 255) / 256) * ((K + 127) / 128), big = ((2l * half + 127) / 128) * ((K + 127) / 128);
-    w = huge * most >= 2048 ? kHuge : big * most >= 512 ? kLarge : kSmall;
+    w = type != 0 && huge * most >= 2048 ? kHuge : big * most >= 512 ? kLarge : kSmall;
     const long tiles = w == kHuge ? huge : w == kLarge ? big : (2l * half / 64) * ((K + 63) / 64);
     long s = (512 + tiles - 1) / tiles;
     if (s > 2) s = (s + 7) / 8 * 8;

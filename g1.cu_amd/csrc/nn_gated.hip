@@ -45,7 +45,7 @@ extern "C" int g1_nn_gated(int type, long M, int K, int F, const void* x, long x
 }
 
 extern "C" long g1_nn_gated_backward_workspace(int type, long M, int K, int F) {
-  return Workspace(type, M, K, Split(M, K, F)).bytes;
+  return Workspace(type, M, K, Split(type, M, K, F)).bytes;
 }
 
 extern "C" int g1_nn_gated_backward(int type, long M, int K, int F, const void* x, long xs, const void* wg, long wgs,
@@ -56,7 +56,7 @@ extern "C" int g1_nn_gated_backward(int type, long M, int K, int F, const void* 
   if (M > 0 && (!x || !wg || !wu || !dy || !ws)) return refuse("a null pointer") ? -1 : 0;
   if (bad_place(type, {x, wg, wu, bg, bu, dy, dx, dwg, dwu, dbg, dbu}) || bad_strides({xs, wgs, wus, dys})) return -1;
   if (!aligned(ws, 16)) return refuse("the workspace is not aligned to 16 bytes") ? -1 : 0;
-  const Split s(M, K, F);
+  const Split s(type, M, K, F);
   const Workspace w(type, M, K, s);
   GatedArgs a{};
   a.M = (int)M, a.K = K, a.F = F, a.x = x, a.wg = wg, a.wu = wu, a.bg = bg, a.bu = bu, a.dy = dy;
